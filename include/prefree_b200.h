@@ -154,6 +154,163 @@ pf_status pf_spmm_f32_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
                           const float *val, int k, double alpha, const float *X,
                           int64_t ldx, double beta, float *Y, int64_t ldy, void *stream);
 
+/* 16-bit values (bit patterns) over wide dense rows, the shape of a routed
+ * model's dispatch and combine: A holds the gates (tokens x slots, a few
+ * non-zeros to a row), X the slots' rows. All k columns in one pass over A;
+ * sums in fp32 in the row's order, rounded once; alpha and beta are rounded to
+ * fp32. Deterministic. Y must not overlap X.                                */
+pf_status pf_spmm_f16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                          const int32_t *row_ptr, const int32_t *col_idx,
+                          const uint16_t *val, int k, double alpha, const uint16_t *X,
+                          int64_t ldx, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_spmm_f16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                          const int64_t *row_ptr, const int32_t *col_idx,
+                          const uint16_t *val, int k, double alpha, const uint16_t *X,
+                          int64_t ldx, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_spmm_bf16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                           const int32_t *row_ptr, const int32_t *col_idx,
+                           const uint16_t *val, int k, double alpha, const uint16_t *X,
+                           int64_t ldx, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_spmm_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                           const int64_t *row_ptr, const int32_t *col_idx,
+                           const uint16_t *val, int k, double alpha, const uint16_t *X,
+                           int64_t ldx, double beta, uint16_t *Y, int64_t ldy, void *stream);
+
+/* ---- sampled dense-dense product: the gradient of an SpMM's values ----------
+ * No counterpart in the reference. dval_j = alpha * <dY[row(j), :], X[col_j, :]>
+ * + beta * dval_j for every non-zero j of the CSR (row_ptr, col_idx): with
+ * Y = A X, the gradient of A's values from that of Y (m x k, lddy >= k) and X
+ * (n x k, ldx >= k). (The gradient of X is A^T dY: pf_spmm_* with the
+ * transposed CSR.) dval is addressed like col_idx, by the absolute row_ptr
+ * values; with beta == 0 it is not read. A non-zero whose column lies outside
+ * [0, n) is flagged and its dval left as it is. fp32 sums in a fixed order,
+ * rounded once. Asynchronous on `stream`.                                   */
+pf_status pf_sddmm_f16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                           const int32_t *row_ptr, const int32_t *col_idx, int k, double alpha,
+                           const uint16_t *dY, int64_t lddy, const uint16_t *X, int64_t ldx,
+                           double beta, uint16_t *dval, void *stream);
+pf_status pf_sddmm_f16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                           const int64_t *row_ptr, const int32_t *col_idx, int k, double alpha,
+                           const uint16_t *dY, int64_t lddy, const uint16_t *X, int64_t ldx,
+                           double beta, uint16_t *dval, void *stream);
+pf_status pf_sddmm_bf16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                            const int32_t *row_ptr, const int32_t *col_idx, int k, double alpha,
+                            const uint16_t *dY, int64_t lddy, const uint16_t *X, int64_t ldx,
+                            double beta, uint16_t *dval, void *stream);
+pf_status pf_sddmm_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                            const int64_t *row_ptr, const int32_t *col_idx, int k, double alpha,
+                            const uint16_t *dY, int64_t lddy, const uint16_t *X, int64_t ldx,
+                            double beta, uint16_t *dval, void *stream);
+
+/* ---- distillation from a teacher's kept logits ------------------------------
+ * No counterpart in the reference. The teacher is a CSR matrix (m tokens x n
+ * vocabulary entries) of the logits it kept, in any order, any number to a
+ * row; the student's logits Z are dense (m x n, ldz >= n). With tau =
+ * temperature, p = softmax(t / tau) over the row's stored logits t and q =
+ * softmax(z / tau) over the student's whole row:
+ *   loss[r]  = weight[r] * sum_j p_j (log p_j - log q_j)
+ *   dZ[r, i] = weight[r] / tau * (q_i - sum of p_j over the entries j of column i)
+ * loss (fp32) and dZ (m x n, lddz >= n, the type of Z) are each optional, one
+ * of them has to be asked for; weight NULL stands for ones. dZ may be Z itself
+ * (same pointer and leading dimension) or must not overlap it. A backward call
+ * of its own is this call with loss = NULL and weight = the losses' gradients
+ * times the weights: it reads Z once too.
+ * An entry with p_j = 0 (a teacher logit of -inf) adds nothing, whatever z_j
+ * is. A row without teacher mass (no entry, or all -inf) has loss 0 and
+ * gradient 0, and so has a row of weight 0, whose Z is not read. A row with
+ * teacher mass where the student has nothing but -inf: loss +inf (times the
+ * weight), q = 0. NaN and +inf logits give NaN. Repeated columns add up; a
+ * column outside [0, n) is flagged in the device error word and ignored.
+ * fp32 arithmetic, the loss's closing terms in double; dZ is rounded once.
+ * Deterministic. Asynchronous on `stream`.                                  */
+pf_status pf_distill_f32_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                             const int32_t *row_ptr, const int32_t *col_idx, const float *val,
+                             double temperature, const float *Z, int64_t ldz,
+                             const float *weight, float *loss, float *dZ, int64_t lddz,
+                             void *stream);
+pf_status pf_distill_f32_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                             const int64_t *row_ptr, const int32_t *col_idx, const float *val,
+                             double temperature, const float *Z, int64_t ldz,
+                             const float *weight, float *loss, float *dZ, int64_t lddz,
+                             void *stream);
+pf_status pf_distill_f16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                             const int32_t *row_ptr, const int32_t *col_idx, const uint16_t *val,
+                             double temperature, const uint16_t *Z, int64_t ldz,
+                             const float *weight, float *loss, uint16_t *dZ, int64_t lddz,
+                             void *stream);
+pf_status pf_distill_f16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                             const int64_t *row_ptr, const int32_t *col_idx, const uint16_t *val,
+                             double temperature, const uint16_t *Z, int64_t ldz,
+                             const float *weight, float *loss, uint16_t *dZ, int64_t lddz,
+                             void *stream);
+pf_status pf_distill_bf16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                              const int32_t *row_ptr, const int32_t *col_idx, const uint16_t *val,
+                              double temperature, const uint16_t *Z, int64_t ldz,
+                              const float *weight, float *loss, uint16_t *dZ, int64_t lddz,
+                              void *stream);
+pf_status pf_distill_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
+                              const int64_t *row_ptr, const int32_t *col_idx, const uint16_t *val,
+                              double temperature, const uint16_t *Z, int64_t ldz,
+                              const float *weight, float *loss, uint16_t *dZ, int64_t lddz,
+                              void *stream);
+
+/* ---- matrix products grouped by rows ----------------------------------------
+ * No counterpart in the reference. Group g owns the rows [group_ptr[g],
+ * group_ptr[g+1]) of X and Y (a row_ptr whose row is a group; group_ptr[0] may
+ * be above 0, groups may be empty, rows in no group are neither read nor
+ * written) and has its own matrix W_g at W + g * stride_w:
+ *   Y[r, :] = alpha * X[r, :] * op(W_g) + beta * Y[r, :]      (n columns)
+ * trans_w != 0: W_g is n x k, Y = X W_g^T (a layer's forward); trans_w == 0:
+ * W_g is k x n, Y = X W_g (the gradient of the layer's input, with n and k
+ * swapped and the same W). X is rows x k, Y rows x n, all row-major with any
+ * leading dimension. group_ptr stays on the device and is never read back; a
+ * group whose pointers decrease or leave [0, rows] is flagged in the device
+ * error word and treated as empty. 16-bit values, fp32 sums, rounded once;
+ * alpha and beta are rounded to fp32; with beta == 0 Y is not read. Y must not
+ * overlap X or W. Deterministic. Asynchronous on `stream`. rows, n, k and
+ * groups are at most 2^31 - 1.                                              */
+pf_status pf_gmm_f16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                         const int32_t *group_ptr, const uint16_t *X, int64_t ldx,
+                         const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,
+                         double alpha, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_gmm_f16_i64(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                         const int64_t *group_ptr, const uint16_t *X, int64_t ldx,
+                         const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,
+                         double alpha, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_gmm_bf16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                          const int32_t *group_ptr, const uint16_t *X, int64_t ldx,
+                          const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,
+                          double alpha, double beta, uint16_t *Y, int64_t ldy, void *stream);
+pf_status pf_gmm_bf16_i64(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                          const int64_t *group_ptr, const uint16_t *X, int64_t ldx,
+                          const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,
+                          double alpha, double beta, uint16_t *Y, int64_t ldy, void *stream);
+/* The gradient of the groups' matrices:
+ *   dW_g = alpha * sum of dY[r, :]^T X[r, :] over g's rows + beta * dW_g
+ * dW_g (n x k, lddw >= k) lies at dW + g * stride_dw elements; dw_bytes = 2:
+ * the type of X, 4: fp32 (to accumulate over micro-batches with beta = 1). An
+ * empty group's dW_g becomes beta * dW_g. Otherwise as pf_gmm_*.            */
+pf_status pf_gmm_wgrad_f16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                               const int32_t *group_ptr, const uint16_t *dY, int64_t lddy,
+                               const uint16_t *X, int64_t ldx, double alpha, double beta,
+                               void *dW, int dw_bytes, int64_t lddw, int64_t stride_dw,
+                               void *stream);
+pf_status pf_gmm_wgrad_f16_i64(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                               const int64_t *group_ptr, const uint16_t *dY, int64_t lddy,
+                               const uint16_t *X, int64_t ldx, double alpha, double beta,
+                               void *dW, int dw_bytes, int64_t lddw, int64_t stride_dw,
+                               void *stream);
+pf_status pf_gmm_wgrad_bf16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                                const int32_t *group_ptr, const uint16_t *dY, int64_t lddy,
+                                const uint16_t *X, int64_t ldx, double alpha, double beta,
+                                void *dW, int dw_bytes, int64_t lddw, int64_t stride_dw,
+                                void *stream);
+pf_status pf_gmm_wgrad_bf16_i64(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
+                                const int64_t *group_ptr, const uint16_t *dY, int64_t lddy,
+                                const uint16_t *X, int64_t ldx, double alpha, double beta,
+                                void *dW, int dw_bytes, int64_t lddw, int64_t stride_dw,
+                                void *stream);
+
 /* ---- fused multiply + all-gather for row-sharded iterated multiplies --------
  * No counterpart in the reference (single GPU only). One step of
  * x_{k+1} = A x_k / ||A x_k|| on this rank's row shard (rows

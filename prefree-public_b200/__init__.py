@@ -46,6 +46,13 @@ EXPORTED = [
     "pf_spmv_f16_i32", "pf_spmv_f16_i64", "pf_spmv_bf16_i32", "pf_spmv_bf16_i64",
     "pf_csr_write", "pf_csr_read", "pf_mmio_read_cached", "pf_mmio_read_pinned",
     "pf_mmio_read_cached_pinned",
+    "pf_spmm_f16_i32", "pf_spmm_f16_i64", "pf_spmm_bf16_i32", "pf_spmm_bf16_i64",
+    "pf_sddmm_f16_i32", "pf_sddmm_f16_i64", "pf_sddmm_bf16_i32", "pf_sddmm_bf16_i64",
+    "pf_distill_f32_i32", "pf_distill_f32_i64", "pf_distill_f16_i32", "pf_distill_f16_i64",
+    "pf_distill_bf16_i32", "pf_distill_bf16_i64",
+    "pf_gmm_f16_i32", "pf_gmm_f16_i64", "pf_gmm_bf16_i32", "pf_gmm_bf16_i64",
+    "pf_gmm_wgrad_f16_i32", "pf_gmm_wgrad_f16_i64", "pf_gmm_wgrad_bf16_i32",
+    "pf_gmm_wgrad_bf16_i64",
 ]
 # the C++ drop-in symbols of include/PreFree.h (mangled)
 CXX_EXPORTED = [
@@ -95,9 +102,26 @@ def _load():
         f = getattr(lib, name)
         f.argtypes = [vp, i64, i64, i64, vp, vp, vp, dbl, vp, dbl, vp, vp]
         f.restype = st
-    for name in ("pf_spmm_f64_i32", "pf_spmm_f64_i64", "pf_spmm_f32_i32", "pf_spmm_f32_i64"):
+    for name in ("pf_spmm_f64_i32", "pf_spmm_f64_i64", "pf_spmm_f32_i32", "pf_spmm_f32_i64",
+                 "pf_spmm_f16_i32", "pf_spmm_f16_i64", "pf_spmm_bf16_i32", "pf_spmm_bf16_i64"):
         f = getattr(lib, name)
         f.argtypes = [vp, i64, i64, i64, vp, vp, vp, C.c_int, dbl, vp, i64, dbl, vp, i64, vp]
+        f.restype = st
+    for t in ("f16_i32", "f16_i64", "bf16_i32", "bf16_i64"):
+        f = getattr(lib, "pf_sddmm_" + t)
+        f.argtypes = [vp, i64, i64, i64, vp, vp, C.c_int, dbl, vp, i64, vp, i64, dbl, vp, vp]
+        f.restype = st
+        f = getattr(lib, "pf_gmm_" + t)
+        f.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, vp, i64, i64, C.c_int, dbl, dbl, vp,
+                      i64, vp]
+        f.restype = st
+        f = getattr(lib, "pf_gmm_wgrad_" + t)
+        f.argtypes = [vp, i64, i64, i64, i64, vp, vp, i64, vp, i64, dbl, dbl, vp, C.c_int, i64,
+                      i64, vp]
+        f.restype = st
+    for t in ("f32_i32", "f32_i64", "f16_i32", "f16_i64", "bf16_i32", "bf16_i64"):
+        f = getattr(lib, "pf_distill_" + t)
+        f.argtypes = [vp, i64, i64, i64, vp, vp, vp, dbl, vp, i64, vp, vp, vp, i64, vp]
         f.restype = st
     for name in ("pf_spmv_dist_f64_i64", "pf_spmv_dist_f64_i32"):
         f = getattr(lib, name)
@@ -254,7 +278,8 @@ def spmv(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, x, y,
 def spmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, X, Y,
          alpha: float = 1.0, beta: float = 0.0, stream=None):
     """Y = alpha*A*X + beta*Y for k = X.shape[1] dense columns (torch CUDA
-    tensors, X n x k and Y m x k, row-major with any row stride >= k)."""
+    tensors, X n x k and Y m x k, row-major with any row stride >= k). 16-bit
+    values take all columns in one pass with fp32 sums."""
     import torch
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
@@ -262,10 +287,134 @@ def spmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, X, Y,
         stream = stream.cuda_stream
     k = int(X.shape[1])
     assert Y.shape[1] == k and X.stride(1) == 1 and Y.stride(1) == 1
-    f = getattr(lib, "pf_spmm_" + _suffix(val.element_size(), row_ptr.element_size()))
+    f = getattr(lib, "pf_spmm_" + _suffix(val.element_size(), row_ptr.element_size(), val.dtype))
     _check(f(handle.ptr, int(m), int(n), int(nnz), _ptr(row_ptr), _ptr(col), _ptr(val), k,
              float(alpha), _ptr(X), int(X.stride(0)), float(beta), _ptr(Y), int(Y.stride(0)),
              C.c_void_p(stream)))
+
+
+def _require(ok: bool, msg: str):
+    if not ok:
+        raise PfError(1, msg)
+
+
+def _rowmajor(t, what: str, rows: int, cols: int, dtype) -> int:
+    """Checks a 2-d CUDA tensor of rows x cols; its leading dimension."""
+    _require(t.is_cuda and t.dim() == 2 and t.dtype == dtype,
+             f"{what}: a 2-d CUDA tensor of {dtype} is wanted")
+    _require(t.shape[0] == rows and t.shape[1] == cols,
+             f"{what}: {tuple(t.shape)} where {(rows, cols)} is wanted")
+    _require(t.stride(1) == 1 or cols <= 1, f"{what}: rows have to be contiguous")
+    return int(t.stride(0)) if rows > 1 else max(int(t.stride(0)), cols)
+
+
+def _index(t, what: str, count: int | None = None, dtypes=("torch.int32", "torch.int64")):
+    """Checks a contiguous 1-d CUDA index tensor."""
+    _require(t.is_cuda and t.dim() == 1 and t.is_contiguous() and str(t.dtype) in dtypes,
+             f"{what}: a contiguous 1-d CUDA tensor of {' or '.join(dtypes)} is wanted")
+    _require(count is None or t.shape[0] >= count, f"{what}: fewer than {count} elements")
+
+
+def _stream(stream):
+    import torch
+    if stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return getattr(stream, "cuda_stream", stream)
+
+
+def sddmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, dY, X, dval,
+          alpha: float = 1.0, beta: float = 0.0, stream=None):
+    """dval_j = alpha*<dY[row(j)], X[col_j]> + beta*dval_j at the non-zeros of
+    the CSR: the gradient of the values of ``spmm`` (16-bit CUDA tensors, dY
+    m x k and X n x k)."""
+    _index(row_ptr, "row_ptr", m + 1)
+    _index(col, "col", nnz, ("torch.int32",))
+    k = int(X.shape[1])
+    ldx, lddy = _rowmajor(X, "X", n, k, dval.dtype), _rowmajor(dY, "dY", m, k, dval.dtype)
+    _require(dval.element_size() == 2 and dval.is_floating_point(), "dval: a 16-bit type is wanted")
+    _require(dval.is_cuda and dval.dim() == 1 and dval.is_contiguous() and dval.shape[0] >= nnz,
+             f"dval: a contiguous CUDA tensor of {nnz} values is wanted")
+    f = getattr(lib, "pf_sddmm_" + _suffix(2, row_ptr.element_size(), dval.dtype))
+    _check(f(handle.ptr, m, n, nnz, row_ptr.data_ptr(), col.data_ptr(), k, alpha, dY.data_ptr(),
+             lddy, X.data_ptr(), ldx, beta, dval.data_ptr(), _stream(stream)))
+
+
+def distill(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, Z, loss=None, dZ=None,
+            weight=None, temperature: float = 1.0, stream=None):
+    """Loss of the student logits Z (m x n) against the teacher's kept logits,
+    a CSR matrix (row_ptr, col, val): loss[r] = weight[r] * KL(p || q) with p =
+    softmax(val / temperature) over row r's entries and q = softmax(Z[r] /
+    temperature), and/or its gradient dZ (which may be Z). ``loss`` and
+    ``weight`` are float32 of m elements; see pf_distill_* in prefree_b200.h
+    for empty rows, infinities and repeated columns. A backward call of its own
+    passes loss=None and weight = the losses' gradients times the weights."""
+    _index(row_ptr, "row_ptr", m + 1)
+    _index(col, "col", nnz, ("torch.int32",))
+    _require(str(Z.dtype) in ("torch.float32", "torch.float16", "torch.bfloat16"),
+             f"Z: {Z.dtype} is not supported")
+    ldz = _rowmajor(Z, "Z", m, n, Z.dtype)
+    _require(val.is_cuda and val.dim() == 1 and val.is_contiguous() and val.dtype == Z.dtype and
+             val.shape[0] >= nnz, f"val: a contiguous CUDA tensor of {nnz} {Z.dtype} is wanted")
+    for t, what in ((loss, "loss"), (weight, "weight")):
+        _require(t is None or (t.is_cuda and t.is_contiguous() and t.numel() == m and
+                               str(t.dtype) == "torch.float32"),
+                 f"{what}: a contiguous float32 CUDA tensor of {m} elements is wanted")
+    lddz = ldz if dZ is None else _rowmajor(dZ, "dZ", m, n, Z.dtype)
+    f = getattr(lib, "pf_distill_" + _suffix(Z.element_size(), row_ptr.element_size(), Z.dtype))
+    _check(f(handle.ptr, m, n, nnz, row_ptr.data_ptr(), col.data_ptr(), val.data_ptr(),
+             temperature, Z.data_ptr(), ldz, _ptr(weight), _ptr(loss), _ptr(dZ), lddz,
+             _stream(stream)))
+
+
+def _matrices(t, what: str, groups: int, rows: int, cols: int) -> tuple[int, int]:
+    """Checks a (groups, rows, cols) CUDA tensor; its leading dimension and
+    the distance between matrices."""
+    _require(t.is_cuda and t.dim() == 3 and tuple(t.shape) == (groups, rows, cols),
+             f"{what}: {tuple(t.shape)} where {(groups, rows, cols)} is wanted")
+    _require(t.stride(2) == 1 or cols <= 1, f"{what}: rows have to be contiguous")
+    ld = int(t.stride(1)) if rows > 1 else max(int(t.stride(1)), cols)
+    return ld, int(t.stride(0))
+
+
+def grouped_mm(handle: Handle, group_ptr, X, W, Y, transpose_w: bool = True, alpha: float = 1.0,
+               beta: float = 0.0, stream=None):
+    """Y[r] = alpha*X[r]*op(W[g]) + beta*Y[r] for the rows r of every group g,
+    group_ptr[g] <= r < group_ptr[g+1] (CUDA tensors; X rows x k and Y rows x n
+    of one 16-bit type). transpose_w: W is (groups, n, k) and op transposes it
+    (a layer's forward); otherwise W is (groups, k, n) (the gradient of the
+    layer's input, with dY for X). Group sizes are not read back to the host."""
+    _index(group_ptr, "group_ptr", 1)
+    groups = group_ptr.shape[0] - 1
+    _require(X.dim() == 2 and Y.dim() == 2, "X, Y: 2-d tensors are wanted")
+    rows, k, n = X.shape[0], X.shape[1], Y.shape[1]
+    _require(X.element_size() == 2 and X.is_floating_point() and W.dtype == X.dtype,
+             "X, W, Y: one 16-bit type is wanted")
+    ldx, ldy = _rowmajor(X, "X", rows, k, X.dtype), _rowmajor(Y, "Y", rows, n, X.dtype)
+    ldw, stride_w = _matrices(W, "W", groups, *((n, k) if transpose_w else (k, n)))
+    f = getattr(lib, "pf_gmm_" + _suffix(2, group_ptr.element_size(), X.dtype))
+    _check(f(handle.ptr, groups, rows, n, k, group_ptr.data_ptr(), X.data_ptr(), ldx,
+             W.data_ptr(), ldw, stride_w, int(transpose_w), alpha, beta, Y.data_ptr(), ldy,
+             _stream(stream)))
+
+
+def grouped_wgrad(handle: Handle, group_ptr, dY, X, dW, alpha: float = 1.0, beta: float = 0.0,
+                  stream=None):
+    """dW[g] = alpha * dY_g^T X_g + beta*dW[g] over the rows of every group g
+    (CUDA tensors; dY rows x n and X rows x k of one 16-bit type, dW (groups, n,
+    k) of that type or float32): the gradient of the W of ``grouped_mm``."""
+    _index(group_ptr, "group_ptr", 1)
+    groups = group_ptr.shape[0] - 1
+    _require(X.dim() == 2 and dY.dim() == 2, "dY, X: 2-d tensors are wanted")
+    rows, k, n = X.shape[0], X.shape[1], dY.shape[1]
+    _require(X.element_size() == 2 and X.is_floating_point() and
+             (dW.dtype == X.dtype or str(dW.dtype) == "torch.float32"),
+             "dY, X: one 16-bit type is wanted, dW: that or float32")
+    ldx, lddy = _rowmajor(X, "X", rows, k, X.dtype), _rowmajor(dY, "dY", rows, n, X.dtype)
+    lddw, stride_dw = _matrices(dW, "dW", groups, n, k)
+    f = getattr(lib, "pf_gmm_wgrad_" + _suffix(2, group_ptr.element_size(), X.dtype))
+    _check(f(handle.ptr, groups, rows, n, k, group_ptr.data_ptr(), dY.data_ptr(), lddy,
+             X.data_ptr(), ldx, alpha, beta, dW.data_ptr(), dW.element_size(), lddw, stride_dw,
+             _stream(stream)))
 
 
 def spmv_dist(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, x, prev_slots,

@@ -1,0 +1,87 @@
+// C-ABI of the distillation loss (distill.cuh).
+#include <algorithm>
+
+#include "distill.cuh"
+#include "pf_handle.cuh"
+
+namespace pf {
+
+template <typename VT, typename IT>
+static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, const IT *row_ptr,
+                                const int32_t *col, const VT *val, double temperature, const VT *Z,
+                                int64_t ldz, const float *weight, float *loss, VT *dZ,
+                                int64_t lddz, cudaStream_t st) {
+  PF_CHECK_ARG(h != nullptr, "null handle");
+  PF_CHECK_ARG(m >= 0 && n >= 0 && nnz >= 0, "negative size (m=%lld n=%lld nnz=%lld)",
+               (long long)m, (long long)n, (long long)nnz);
+  PF_CHECK_ARG(temperature > 0.0 && temperature <= 1e30 && temperature >= 1e-30,
+               "temperature %g outside [1e-30, 1e30]", temperature);
+  if (m == 0) return PF_OK;
+  PF_CHECK_ARG(n <= (int64_t)INT32_MAX, "n must fit int32 column indices");
+  PF_CHECK_ARG(loss || dZ, "neither loss nor dZ is asked for");
+  PF_CHECK_ARG(row_ptr, "null row_ptr");
+  PF_CHECK_ARG(nnz == 0 || (col && val), "null col/val with nnz > 0");
+  PF_CHECK_ARG(nnz == 0 || n > 0, "nnz > 0 needs n > 0 (column indices lie in [0, n))");
+  PF_CHECK_ARG(n == 0 || Z, "null Z");
+  PF_CHECK_ARG(sizeof(IT) == 8 || nnz <= INT32_MAX, "int32 row_ptr cannot index nnz=%lld",
+               (long long)nnz);
+  PF_CHECK_ARG(ldz >= n && (!dZ || lddz >= n), "leading dimension below n");
+  PF_CHECK_ARG((const void *)dZ != (const void *)Z || lddz == ldz,
+               "dZ in Z's place needs lddz == ldz");
+  PF_CHECK_ARG(((uintptr_t)row_ptr % sizeof(IT)) == 0 && ((uintptr_t)col % 4) == 0 &&
+                   ((uintptr_t)val % sizeof(VT)) == 0 && ((uintptr_t)Z % sizeof(VT)) == 0 &&
+                   ((uintptr_t)dZ % sizeof(VT)) == 0 && ((uintptr_t)weight % 4) == 0 &&
+                   ((uintptr_t)loss % 4) == 0,
+               "arrays must be aligned to their element size");
+  int cur = 0;
+  PF_CUDA_TRY(cudaGetDevice(&cur));
+  PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
+  DistillParams<VT, IT> p;
+  p.m = m;
+  p.n = n;
+  p.nnz = nnz;
+  p.row_ptr = row_ptr;
+  p.col = col;
+  p.val = val;
+  p.Z = Z;
+  p.ldz = ldz;
+  p.weight = weight;
+  p.loss = loss;
+  p.dZ = dZ;
+  p.lddz = lddz;
+  p.inv_tau = (float)(1.0 / temperature);
+  p.err = h->err;
+  const unsigned grid = (unsigned)std::min<int64_t>(m, INT32_MAX);
+  distill_kernel<VT, IT, 512><<<grid, 512, 0, st>>>(p);
+  count_launches(1);
+  PF_CUDA_TRY(cudaGetLastError());
+  return PF_OK;
+}
+
+}  // namespace pf
+
+using namespace pf;
+
+extern "C" {
+
+// 16-bit values cross the C ABI as their raw bit patterns (uint16_t)
+#define PF_DEFINE_DISTILL(SUFFIX, VT, CT, IT)                                              \
+  pf_status pf_distill_##SUFFIX(pf_handle h, int64_t m, int64_t n, int64_t nnz,            \
+                                const IT *row_ptr, const int32_t *col_idx, const CT *val,  \
+                                double temperature, const CT *Z, int64_t ldz,              \
+                                const float *weight, float *loss, CT *dZ, int64_t lddz,    \
+                                void *stream) {                                            \
+    return launch_distill<VT, IT>(h, m, n, nnz, row_ptr, col_idx,                          \
+                                  reinterpret_cast<const VT *>(val), temperature,          \
+                                  reinterpret_cast<const VT *>(Z), ldz, weight, loss,      \
+                                  reinterpret_cast<VT *>(dZ), lddz, (cudaStream_t)stream); \
+  }
+
+PF_DEFINE_DISTILL(f32_i32, float, float, int32_t)
+PF_DEFINE_DISTILL(f32_i64, float, float, int64_t)
+PF_DEFINE_DISTILL(f16_i32, __half, uint16_t, int32_t)
+PF_DEFINE_DISTILL(f16_i64, __half, uint16_t, int64_t)
+PF_DEFINE_DISTILL(bf16_i32, __nv_bfloat16, uint16_t, int32_t)
+PF_DEFINE_DISTILL(bf16_i64, __nv_bfloat16, uint16_t, int64_t)
+
+}  // extern "C"
