@@ -1,10 +1,138 @@
 // C-ABI of the grouped matrix products.
 #include <algorithm>
+#include <type_traits>
 
 #include "gmm_simt.cuh"
+#include "gmm_tc.cuh"
 #include "pf_handle.cuh"
 
 namespace pf {
+
+// cuTensorMapEncodeTiled, looked up at run time (the library does not link
+// against the driver); null where there is none
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                             const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) !=
+            cudaSuccess || r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+
+// A map of `planes` row-major matrices (rows x cols, leading dimension ld,
+// `plane` elements apart; planes = 0: one matrix, a 2-d map) for boxes of 64
+// columns x box_rows rows, 128-byte swizzle, zeros outside.
+template <typename VT>
+static pf_status encode(CUtensorMap *map, const VT *base, int64_t cols, int64_t rows, int64_t ld,
+                        int64_t planes, int64_t plane, int box_rows) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available");
+    return PF_ERR_CUDA;
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * sizeof(VT), (cuuint64_t)plane * sizeof(VT)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+  const CUtensorMapDataType type = std::is_same<VT, __half>::value
+                                       ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = fn(map, type, planes ? 3 : 2, const_cast<VT *>(base), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled: error %d", (int)r);
+    return PF_ERR_CUDA;
+  }
+  return PF_OK;
+}
+
+// what a tensor map takes: 16-byte aligned base and strides
+template <typename VT>
+static bool tma_ready(const VT *base, int64_t ld, int64_t plane = 0) {
+  return ((uintptr_t)base % 16) == 0 && ld % 8 == 0 && plane % 8 == 0 && ld < (1LL << 38) &&
+         plane < (1LL << 38);
+}
+
+template <int MODE, int CG, int BN, bool BF16, typename IT, typename OT>
+static pf_status launch_tc(pf_handle h, const GmmMaps &maps, const GmmTcParams<IT, OT> &p,
+                           cudaStream_t st) {
+  using Cfg = GmmCfg<MODE, CG, BN>;
+  auto kern = gmm_tc_kernel<MODE, CG, BN, BF16, IT, OT>;
+  static bool ready[64] = {};  // the attribute is set once per device
+  bool &done = ready[h->device % 64];
+  if (!done) {
+    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    done = true;
+  }
+  // no more tiles than whole ones and one partial one to a group
+  const int64_t ti = ceil_div(p.ni, Cfg::TI);
+  const int64_t tiles = MODE == GMM_DW ? p.groups * ti * ceil_div(p.nj, BN)
+                                       : (p.rows / BN + std::min(p.groups, p.rows)) * ti;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, h->num_sms / CG) * CG));
+  cfg.blockDim = dim3(Cfg::NT);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, maps, p));
+  count_launches(1);
+  return PF_OK;
+}
+
+template <int MODE, typename VT, typename IT>
+static pf_status product_tc(pf_handle h, const VT *X, int64_t ldx, const VT *W, int64_t ldw,
+                            int64_t stride_w, int64_t k, GmmTcParams<IT, VT> p, cudaStream_t st) {
+  constexpr bool BF16 = std::is_same<VT, __nv_bfloat16>::value;
+  // tiles as wide as a group's rows on average
+  const int64_t avg = p.rows / std::min(p.groups, p.rows);
+  const int bn = avg > 128 ? (p.ni > 128 ? 256 : 128) : avg > 64 ? 128 : avg > 32 ? 64 : 32;
+  const int box = bn == 256 ? 32 : bn < 32 ? bn : 32;
+  const bool fwd = MODE == GMM_FWD;
+  GmmMaps maps = {};
+  p.group_step = stride_w != 0 || p.groups == 1;
+  const int64_t planes = p.group_step ? p.groups : 1;
+  const int64_t plane = p.groups == 1 || !p.group_step ? (fwd ? p.ni : k) * ldw : stride_w;
+  pf_status s = encode(&maps.a, W, fwd ? k : p.ni, fwd ? p.ni : k, ldw, planes, plane,
+                       fwd ? 128 : 64);
+  if (s != PF_OK) return s;
+  s = encode(&maps.b, X, k, p.rows, ldx, 0, 0, box);
+  if (s != PF_OK) return s;
+  switch (bn) {
+    case 256: return launch_tc<MODE, 2, 256, BF16>(h, maps, p, st);
+    case 128: return launch_tc<MODE, 1, 128, BF16>(h, maps, p, st);
+    case 64: return launch_tc<MODE, 1, 64, BF16>(h, maps, p, st);
+    default: return launch_tc<MODE, 1, 32, BF16>(h, maps, p, st);
+  }
+}
+
+template <typename VT, typename OT, typename IT>
+static pf_status wgrad_tc(pf_handle h, const VT *dY, int64_t lddy, const VT *X, int64_t ldx,
+                          const GmmTcParams<IT, OT> &p, cudaStream_t st) {
+  constexpr bool BF16 = std::is_same<VT, __nv_bfloat16>::value;
+  GmmMaps maps = {};
+  CUtensorMap *m[3][2] = {{&maps.a, &maps.b}, {&maps.a8, &maps.b8}, {&maps.a1, &maps.b1}};
+  const int box[3] = {64, 8, 1};
+  for (int i = 0; i < 3; ++i) {
+    pf_status s = encode(m[i][0], X, p.ni, p.rows, ldx, 0, 0, box[i]);
+    if (s != PF_OK) return s;
+    s = encode(m[i][1], dY, p.nj, p.rows, lddy, 0, 0, box[i]);
+    if (s != PF_OK) return s;
+  }
+  if (p.ni > 128 && p.nj > 128) return launch_tc<GMM_DW, 2, 256, BF16>(h, maps, p, st);
+  return launch_tc<GMM_DW, 1, 128, BF16>(h, maps, p, st);
+}
 
 template <typename VT, typename IT>
 static pf_status launch_gmm(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
@@ -22,7 +150,8 @@ static pf_status launch_gmm(pf_handle h, int64_t groups, int64_t rows, int64_t n
   PF_CHECK_ARG(k == 0 || (X && W), "null X/W with k > 0");
   const int64_t wcols = trans_w ? k : n, wrows = trans_w ? n : k;
   PF_CHECK_ARG(ldx >= k && ldw >= wcols && ldy >= n, "leading dimension below the row's length");
-  PF_CHECK_ARG(groups == 1 || wrows == 0 || stride_w >= (wrows - 1) * ldw + wcols,
+  PF_CHECK_ARG(groups == 1 || wrows == 0 || stride_w == 0 ||
+                   stride_w >= (wrows - 1) * ldw + wcols,
                "stride_w below one matrix");
   PF_CHECK_ARG(((uintptr_t)ptr % sizeof(IT)) == 0 && ((uintptr_t)X % sizeof(VT)) == 0 &&
                    ((uintptr_t)W % sizeof(VT)) == 0 && ((uintptr_t)Y % sizeof(VT)) == 0,
@@ -30,6 +159,12 @@ static pf_status launch_gmm(pf_handle h, int64_t groups, int64_t rows, int64_t n
   int cur = 0;
   PF_CUDA_TRY(cudaGetDevice(&cur));
   PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
+  if (k > 0 && tma_ready(X, ldx) && tma_ready(W, ldw, groups > 1 ? stride_w : 0)) {
+    GmmTcParams<IT, VT> p{groups, rows, (int)n, 0, (int)k, 1, ptr, Y, ldy, 0,
+                          (float)alpha, (float)beta, h->err};
+    return trans_w ? product_tc<GMM_FWD>(h, X, ldx, W, ldw, stride_w, k, p, st)
+                   : product_tc<GMM_DX>(h, X, ldx, W, ldw, stride_w, k, p, st);
+  }
   GmmSimtParams<VT, VT, IT> p{groups, rows, n,   k,   ptr, X,
                               ldx,    W,    ldw, stride_w, Y,   ldy,
                               0,      (float)alpha, (float)beta, h->err};
@@ -66,6 +201,11 @@ static pf_status launch_wgrad(pf_handle h, int64_t groups, int64_t rows, int64_t
   int cur = 0;
   PF_CUDA_TRY(cudaGetDevice(&cur));
   PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
+  if (rows > 0 && tma_ready(X, ldx) && tma_ready(dY, lddy)) {
+    GmmTcParams<IT, OT> p{groups, rows, (int)k, (int)n, 0, 1, ptr, dW, lddw, stride_dw,
+                          (float)alpha, (float)beta, h->err};
+    return wgrad_tc<VT>(h, dY, lddy, X, ldx, p, st);
+  }
   GmmSimtParams<VT, OT, IT> p{groups, rows, n,   k, ptr, dY,
                               lddy,   X,    ldx, 0, dW,  lddw,
                               stride_dw, (float)alpha, (float)beta, h->err};
