@@ -60,6 +60,11 @@ static bool tma_ready(const VT *base, int64_t ld, int64_t plane = 0) {
          plane < (1LL << 38);
 }
 
+template <typename OT>
+static bool rows_aligned(const OT *c, int64_t ld, int64_t plane) {
+  return ((uintptr_t)c % 16) == 0 && ld * sizeof(OT) % 16 == 0 && plane * sizeof(OT) % 16 == 0;
+}
+
 template <int MODE, int CG, int BN, bool BF16, typename IT, typename OT>
 static pf_status launch_tc(pf_handle h, const GmmMaps &maps, const GmmTcParams<IT, OT> &p,
                            cudaStream_t st) {
@@ -161,7 +166,8 @@ static pf_status launch_gmm(pf_handle h, int64_t groups, int64_t rows, int64_t n
   PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
   if (k > 0 && tma_ready(X, ldx) && tma_ready(W, ldw, groups > 1 ? stride_w : 0)) {
     GmmTcParams<IT, VT> p{groups, rows, (int)n, 0, (int)k, 1, ptr, Y, ldy, 0,
-                          (float)alpha, (float)beta, h->err};
+                          (float)alpha, (float)beta, rows_aligned(Y, ldy, 0),
+                          beta == 0.0 && rows_aligned(Y, ldy, 0), h->err};
     return trans_w ? product_tc<GMM_FWD>(h, X, ldx, W, ldw, stride_w, k, p, st)
                    : product_tc<GMM_DX>(h, X, ldx, W, ldw, stride_w, k, p, st);
   }
@@ -203,7 +209,8 @@ static pf_status launch_wgrad(pf_handle h, int64_t groups, int64_t rows, int64_t
   PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
   if (rows > 0 && tma_ready(X, ldx) && tma_ready(dY, lddy)) {
     GmmTcParams<IT, OT> p{groups, rows, (int)k, (int)n, 0, 1, ptr, dW, lddw, stride_dw,
-                          (float)alpha, (float)beta, h->err};
+                          (float)alpha, (float)beta, rows_aligned(dW, lddw, stride_dw),
+                          beta == 0.0 && rows_aligned(dW, lddw, stride_dw), h->err};
     return wgrad_tc<VT>(h, dY, lddy, X, ldx, p, st);
   }
   GmmSimtParams<VT, OT, IT> p{groups, rows, n,   k, ptr, dY,

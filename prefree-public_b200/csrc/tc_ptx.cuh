@@ -169,5 +169,31 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// lanes 0-15 from `addr`'s lane on, 32 columns, as fragments: registers 4b and
+// 4b + 1 hold columns 8b + 2 (lane mod 4) and the next of lane `lane / 4`,
+// 4b + 2 and 4b + 3 those of lane `lane / 4 + 8`. Wait before use.
+__device__ __forceinline__ void tmem_load16x256b_x4(uint32_t addr, float (&v)[16]) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// four 8 x 8 matrices of 16-bit values, each stored transposed; lane l gives
+// the address of line l mod 8 of matrix l / 8
+__device__ __forceinline__ void store_matrices_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                 uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr),
+               "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
 }  // namespace tc
 }  // namespace pf
