@@ -225,6 +225,21 @@ struct GmmTiles {
   }
 };
 
+// A panel of `valid` < 64 rows from `row` on, filled up to a multiple of 16 with
+// zero rows (boxes at row `outside`, past the array).
+template <int CG>
+__device__ __forceinline__ void load_ragged(uint32_t dst, const CUtensorMap *m8,
+                                            const CUtensorMap *m1, uint32_t bar, int c, int row,
+                                            int valid, int outside) {
+  for (int r = 0; r < (valid + 15) / 16 * 16; r += 8) {
+    if (r + 8 <= valid || r >= valid)
+      tc::load_2d<CG>(dst + r * 128, m8, bar, c, r < valid ? row + r : outside);
+    else
+      for (int q = r; q < r + 8; ++q)
+        tc::load_2d<CG>(dst + q * 128, m1, bar, c, q < valid ? row + q : outside);
+  }
+}
+
 // columns that the matrix instruction computes for jn outputs
 template <int CG>
 __device__ __forceinline__ int instr_cols(int jn) {
@@ -264,8 +279,9 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   tc::fence_after_sync();
   const uint32_t tmem = tmem_base;
 
-  auto wait = [&](uint64_t *bar, uint32_t parity) {
-    if (ptx::mbar_wait_bounded(bar, parity, GMM_WAIT_NS)) return true;
+  // called by whole warps
+  auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+    if (__all_sync(~0u, ptx::mbar_wait_bounded(bar, parity, GMM_WAIT_NS))) return true;
     atomicOr(P.err, PF_DEVERR_WAIT_TIMEOUT);
     dead = 1;
     return false;
@@ -274,6 +290,8 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   GmmTiles<MODE, CG, BN, IT, OT> tiles(P);
   GmmTile t;
   if (wid == 0) {  // ---- copies
+    const uint32_t full_at = CG == 2 ? tc::map_rank(tc::smem_addr(&full[0]), 0)
+                                     : tc::smem_addr(&full[0]);
     uint32_t it = 0;
     bool ok = true;
     while (ok && tiles.next(&t)) {
@@ -281,41 +299,35 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       const int ncols = instr_cols<CG>(t.jn), half = ncols / CG;
       const int gw = (int)t.g * P.group_step;
       const int ia = t.i0 + (int)rank * 128;
-      if (lane == 0) {
-        for (int kb = 0; kb < nb; ++kb, ++it) {
-          const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
-          if (!wait(&empty[s], ph ^ 1)) {
-            ok = false;
-            break;
-          }
+      for (int kb = 0; kb < nb; ++kb, ++it) {
+        const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
+        if (!wait(&empty[s], ph ^ 1)) {
+          ok = false;
+          break;
+        }
+        if (tc::elect()) {
           const uint32_t sa = stage0 + s * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
-          const uint32_t bar = CG == 2 ? tc::map_rank(tc::smem_addr(&full[s]), 0)
-                                       : tc::smem_addr(&full[s]);
+          const uint32_t bar = full_at + s * 8;
           if constexpr (MODE == GMM_DW) {
             const int left = t.np - kb * 64;
             const int valid = left < 64 ? left : 64, r16 = (valid + 15) / 16 * 16;
             const int panels_b = (half + 63) / 64;
             if (rank == 0)
               ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * (2 + panels_b) * r16 * 128));
-            const int row = (int)t.p0 + kb * 64, outside = (int)P.rows;
+            const int row = (int)t.p0 + kb * 64;
             const int jb = (int)t.j0 + (int)rank * half;
-            for (int x = 0; x < 2 + panels_b; ++x) {
-              const bool is_a = x < 2;
-              const uint32_t dst = is_a ? sa + x * 8192 : sb + (x - 2) * 8192;
-              const int c = is_a ? ia + x * 64 : jb + (x - 2) * 64;
-              if (valid == 64) {
-                tc::load_2d<CG>(dst, is_a ? &M.a : &M.b, bar, c, row);
-                continue;
-              }
-              for (int r = 0; r < r16; r += 8) {
-                if (r + 8 <= valid || r >= valid)
-                  tc::load_2d<CG>(dst + r * 128, is_a ? &M.a8 : &M.b8, bar, c,
-                                  r < valid ? row + r : outside);
-                else
-                  for (int q = r; q < r + 8; ++q)
-                    tc::load_2d<CG>(dst + q * 128, is_a ? &M.a1 : &M.b1, bar, c,
-                                    q < valid ? row + q : outside);
-              }
+            if (valid == 64) {
+              tc::load_2d<CG>(sa, &M.a, bar, ia, row);
+              tc::load_2d<CG>(sa + 8192, &M.a, bar, ia + 64, row);
+              for (int x = 0; x < panels_b; ++x)
+                tc::load_2d<CG>(sb + x * 8192, &M.b, bar, jb + x * 64, row);
+            } else {
+              for (int x = 0; x < 2; ++x)
+                load_ragged<CG>(sa + x * 8192, &M.a8, &M.a1, bar, ia + x * 64, row, valid,
+                                (int)P.rows);
+              for (int x = 0; x < panels_b; ++x)
+                load_ragged<CG>(sb + x * 8192, &M.b8, &M.b1, bar, jb + x * 64, row, valid,
+                                (int)P.rows);
             }
           } else {
             const int boxes = (half + Cfg::BOX - 1) / Cfg::BOX;
@@ -333,14 +345,12 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
               tc::load_2d<CG>(sb + x * Cfg::BOX * 128, &M.b, bar, kb * 64, row + x * Cfg::BOX);
           }
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(~0u, (int)ok, 0);
-      it = __shfl_sync(~0u, it, 0);
     }
     // every stage read: no completion is on its way to a CTA that has ended
-    if (lane == 0)
-      for (int x = 0; ok && x < Cfg::STAGES; ++x, ++it)
-        ok = wait(&empty[it % Cfg::STAGES], (it / Cfg::STAGES & 1) ^ 1);
+    for (int x = 0; ok && x < Cfg::STAGES; ++x, ++it)
+      ok = wait(&empty[it % Cfg::STAGES], (it / Cfg::STAGES & 1) ^ 1);
   } else if (wid == 1 && rank == 0) {  // ---- matrix instructions
     uint32_t it = 0, tile = 0;
     bool ok = true;
@@ -349,32 +359,33 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       if (nb == 0) continue;
       const uint32_t buf = tile & 1, aph = tile >> 1 & 1;
       ++tile;
-      if (lane == 0) {
-        const uint32_t idesc = tc::instr_desc(BF16, MODE != GMM_FWD, MODE == GMM_DW, 128 * CG,
-                                              (uint32_t)instr_cols<CG>(t.jn));
-        ok = wait(&acc_empty[buf], aph ^ 1);
+      const uint32_t idesc = tc::instr_desc(BF16, MODE != GMM_FWD, MODE == GMM_DW, 128 * CG,
+                                            (uint32_t)instr_cols<CG>(t.jn));
+      ok = wait(&acc_empty[buf], aph ^ 1);
+      tc::fence_after_sync();
+      const uint32_t d = tmem + buf * BN;
+      for (int kb = 0; ok && kb < nb; ++kb, ++it) {
+        const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
+        if (!wait(&full[s], ph)) {
+          ok = false;
+          break;
+        }
         tc::fence_after_sync();
-        const uint32_t d = tmem + buf * BN;
-        for (int kb = 0; ok && kb < nb; ++kb, ++it) {
-          const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
-          if (!wait(&full[s], ph)) {
-            ok = false;
-            break;
-          }
-          tc::fence_after_sync();
+        if (tc::elect()) {
           const uint32_t sa = stage0 + s * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
           const uint64_t da = tc::operand_desc(sa, 8192), db = tc::operand_desc(sb, 8192);
-          const int left = t.np - kb * 64, steps = left < 64 ? (left + 15) / 16 : 4;
+          const int left = t.np - kb * 64;
           // 16 along p: 32 bytes of a line, or two atoms of eight lines
           constexpr int STEP_A = MODE == GMM_FWD ? 2 : 128, STEP_B = MODE == GMM_DW ? 128 : 2;
-          for (int q = 0; q < steps; ++q)
-            tc::mma<CG>(d, da + q * STEP_A, db + q * STEP_B, idesc, kb + q > 0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q * 16 < left)
+              tc::mma<CG>(d, da + q * STEP_A, db + q * STEP_B, idesc, kb + q > 0);
           tc::commit<CG>(&empty[s]);
+          if (kb + 1 == nb) tc::commit<CG>(&acc_full[buf]);
         }
-        if (ok) tc::commit<CG>(&acc_full[buf]);
+        __syncwarp();
       }
-      ok = __shfl_sync(~0u, (int)ok, 0);
-      it = __shfl_sync(~0u, it, 0);
     }
   } else if (wid >= 2) {  // ---- accumulator to C
     const int quad = wid & 3;  // the tensor memory lanes that this warp may read
@@ -388,7 +399,6 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       if (sum) {
         ++tile;
         ok = wait(&acc_full[buf], aph);
-        ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after_sync();
       }

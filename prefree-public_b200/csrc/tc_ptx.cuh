@@ -12,6 +12,18 @@ namespace tc {
 
 using ptx::smem_addr;
 
+// True in one lane of a converged warp. Tensor copies and matrix instructions
+// are issued under it, in code that the whole warp walks: behind a comparison
+// of the lane number instead, each such instruction cost about 125 cycles
+// (its operands live in the warp's uniform registers).
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
