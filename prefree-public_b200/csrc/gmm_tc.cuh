@@ -97,7 +97,17 @@ template <typename OT>
 __device__ __forceinline__ void store_pairs(const uint8_t *stage, OT *c, int64_t ldc, int ni,
                                             int nj) {
   const int lane = threadIdx.x & 31, x = lane & 3;
+  if (ni == 32 && nj == 32) {
+    const uint8_t *from = stage + (lane >> 2) * 80 + x * 16;
+    OT *p = c + (lane >> 2) * ldc + x * 8;
+    uint4 v[4];
 #pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4 *>(from + q * 640);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4 *>(p + q * 8 * ldc) = v[q];
+    return;
+  }
+#pragma unroll 1
   for (int q = 0; q < 4; ++q) {
     const int j = q * 8 + (lane >> 2);
     if (j >= nj) continue;
