@@ -280,46 +280,80 @@ def spmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, X, Y,
     """Y = alpha*A*X + beta*Y for k = X.shape[1] dense columns (torch CUDA
     tensors, X n x k and Y m x k, row-major with any row stride >= k). 16-bit
     values take all columns in one pass with fp32 sums."""
+    k = int(X.shape[1])
+    if val.element_size() == 2:
+        f, dtype = _entry("spmm", val.dtype, row_ptr.dtype), val.dtype
+        ldx, ldy = _ld(X, "X", n, k, dtype), _ld(Y, "Y", m, k, dtype)
+        _check(f(handle.ptr, m, n, nnz, _flat(row_ptr, "row_ptr", m + 1, row_ptr.dtype),
+                 _flat(col, "col", nnz, _I32), _flat(val, "val", nnz, dtype), k, alpha,
+                 X.data_ptr(), ldx, beta, Y.data_ptr(), ldy, _stream(stream, X)))
+        return
     import torch
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
     elif hasattr(stream, "cuda_stream"):
         stream = stream.cuda_stream
-    k = int(X.shape[1])
     assert Y.shape[1] == k and X.stride(1) == 1 and Y.stride(1) == 1
-    f = getattr(lib, "pf_spmm_" + _suffix(val.element_size(), row_ptr.element_size(), val.dtype))
+    f = getattr(lib, "pf_spmm_" + _suffix(val.element_size(), row_ptr.element_size()))
     _check(f(handle.ptr, int(m), int(n), int(nnz), _ptr(row_ptr), _ptr(col), _ptr(val), k,
              float(alpha), _ptr(X), int(X.stride(0)), float(beta), _ptr(Y), int(Y.stride(0)),
              C.c_void_p(stream)))
 
 
-def _require(ok: bool, msg: str):
-    if not ok:
-        raise PfError(1, msg)
+# The checks below cost a few microseconds a call, about what a launch does:
+# one expression on the good path, its message built only on refusal.
+_ENTRIES: dict = {}
+_I32 = _F32 = _current_stream = None  # set by the first _entry (torch is imported then)
 
 
-def _rowmajor(t, what: str, rows: int, cols: int, dtype) -> int:
-    """Checks a 2-d CUDA tensor of rows x cols; its leading dimension."""
-    _require(t.is_cuda and t.dim() == 2 and t.dtype == dtype,
-             f"{what}: a 2-d CUDA tensor of {dtype} is wanted")
-    _require(t.shape[0] == rows and t.shape[1] == cols,
-             f"{what}: {tuple(t.shape)} where {(rows, cols)} is wanted")
-    _require(t.stride(1) == 1 or cols <= 1, f"{what}: rows have to be contiguous")
-    return int(t.stride(0)) if rows > 1 else max(int(t.stride(0)), cols)
+def _entry(name: str, dtype, index_dtype):
+    """The C entry pf_<name>_<value>_<index> for two torch dtypes."""
+    f = _ENTRIES.get((name, dtype, index_dtype))
+    return f if f is not None else _new_entry(name, dtype, index_dtype)
 
 
-def _index(t, what: str, count: int | None = None, dtypes=("torch.int32", "torch.int64")):
-    """Checks a contiguous 1-d CUDA index tensor."""
-    _require(t.is_cuda and t.dim() == 1 and t.is_contiguous() and str(t.dtype) in dtypes,
-             f"{what}: a contiguous 1-d CUDA tensor of {' or '.join(dtypes)} is wanted")
-    _require(count is None or t.shape[0] >= count, f"{what}: fewer than {count} elements")
-
-
-def _stream(stream):
+def _new_entry(name: str, dtype, index_dtype):
+    global _I32, _F32, _current_stream
     import torch
+    v = {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}.get(dtype)
+    i = {torch.int32: "i32", torch.int64: "i64"}.get(index_dtype)
+    f = getattr(lib, f"pf_{name}_{v}_{i}", None)
+    if f is None:
+        raise PfError(1, f"{name}: values of {dtype} with indices of {index_dtype}")
+    _I32, _F32 = torch.int32, torch.float32
+    # the current stream's handle without building a Stream object, where
+    # this torch has such a call
+    _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    _ENTRIES[(name, dtype, index_dtype)] = f
+    return f
+
+
+def _stream(stream, t) -> int:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return _current_stream(t.get_device())
     return getattr(stream, "cuda_stream", stream)
+
+
+def _ld(t, what: str, rows: int, cols: int, dtype) -> int:
+    """The leading dimension of a row-major rows x cols CUDA tensor."""
+    if t.shape != (rows, cols) or t.dtype != dtype or not t.is_cuda:
+        raise PfError(1, f"{what}: a CUDA tensor of {(rows, cols)} {dtype} is wanted, not of "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise PfError(1, f"{what}: rows have to be contiguous")
+    return ld if rows > 1 else max(ld, cols)
+
+
+def _flat(t, what: str, least: int, dtype, exact: bool = False) -> int:
+    """The address of a contiguous 1-d CUDA tensor of at least (or exactly)
+    `least` elements."""
+    if not t.is_cuda or t.dtype != dtype or t.dim() != 1 or t.shape[0] < least or \
+            (exact and t.shape[0] != least) or not t.is_contiguous():
+        raise PfError(1, f"{what}: a contiguous 1-d CUDA tensor of {'' if exact else 'at least '}"
+                         f"{least} {dtype} is wanted, not {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def sddmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, dY, X, dval,
@@ -327,16 +361,12 @@ def sddmm(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, dY, X, dval,
     """dval_j = alpha*<dY[row(j)], X[col_j]> + beta*dval_j at the non-zeros of
     the CSR: the gradient of the values of ``spmm`` (16-bit CUDA tensors, dY
     m x k and X n x k)."""
-    _index(row_ptr, "row_ptr", m + 1)
-    _index(col, "col", nnz, ("torch.int32",))
-    k = int(X.shape[1])
-    ldx, lddy = _rowmajor(X, "X", n, k, dval.dtype), _rowmajor(dY, "dY", m, k, dval.dtype)
-    _require(dval.element_size() == 2 and dval.is_floating_point(), "dval: a 16-bit type is wanted")
-    _require(dval.is_cuda and dval.dim() == 1 and dval.is_contiguous() and dval.shape[0] >= nnz,
-             f"dval: a contiguous CUDA tensor of {nnz} values is wanted")
-    f = getattr(lib, "pf_sddmm_" + _suffix(2, row_ptr.element_size(), dval.dtype))
-    _check(f(handle.ptr, m, n, nnz, row_ptr.data_ptr(), col.data_ptr(), k, alpha, dY.data_ptr(),
-             lddy, X.data_ptr(), ldx, beta, dval.data_ptr(), _stream(stream)))
+    f = _entry("sddmm", dval.dtype, row_ptr.dtype)
+    k = X.shape[-1]
+    ldx, lddy = _ld(X, "X", n, k, dval.dtype), _ld(dY, "dY", m, k, dval.dtype)
+    _check(f(handle.ptr, m, n, nnz, _flat(row_ptr, "row_ptr", m + 1, row_ptr.dtype),
+             _flat(col, "col", nnz, _I32), k, alpha, dY.data_ptr(), lddy, X.data_ptr(), ldx,
+             beta, _flat(dval, "dval", nnz, dval.dtype), _stream(stream, X)))
 
 
 def distill(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, Z, loss=None, dZ=None,
@@ -348,32 +378,26 @@ def distill(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, Z, loss
     ``weight`` are float32 of m elements; see pf_distill_* in prefree_b200.h
     for empty rows, infinities and repeated columns. A backward call of its own
     passes loss=None and weight = the losses' gradients times the weights."""
-    _index(row_ptr, "row_ptr", m + 1)
-    _index(col, "col", nnz, ("torch.int32",))
-    _require(str(Z.dtype) in ("torch.float32", "torch.float16", "torch.bfloat16"),
-             f"Z: {Z.dtype} is not supported")
-    ldz = _rowmajor(Z, "Z", m, n, Z.dtype)
-    _require(val.is_cuda and val.dim() == 1 and val.is_contiguous() and val.dtype == Z.dtype and
-             val.shape[0] >= nnz, f"val: a contiguous CUDA tensor of {nnz} {Z.dtype} is wanted")
-    for t, what in ((loss, "loss"), (weight, "weight")):
-        _require(t is None or (t.is_cuda and t.is_contiguous() and t.numel() == m and
-                               str(t.dtype) == "torch.float32"),
-                 f"{what}: a contiguous float32 CUDA tensor of {m} elements is wanted")
-    lddz = ldz if dZ is None else _rowmajor(dZ, "dZ", m, n, Z.dtype)
-    f = getattr(lib, "pf_distill_" + _suffix(Z.element_size(), row_ptr.element_size(), Z.dtype))
-    _check(f(handle.ptr, m, n, nnz, row_ptr.data_ptr(), col.data_ptr(), val.data_ptr(),
-             temperature, Z.data_ptr(), ldz, _ptr(weight), _ptr(loss), _ptr(dZ), lddz,
-             _stream(stream)))
+    dtype = Z.dtype
+    f = _entry("distill", dtype, row_ptr.dtype)
+    ldz = _ld(Z, "Z", m, n, dtype)
+    _check(f(handle.ptr, m, n, nnz, _flat(row_ptr, "row_ptr", m + 1, row_ptr.dtype),
+             _flat(col, "col", nnz, _I32), _flat(val, "val", nnz, dtype), temperature,
+             Z.data_ptr(), ldz, None if weight is None else _flat(weight, "weight", m, _F32, True),
+             None if loss is None else _flat(loss, "loss", m, _F32, True),
+             None if dZ is None else dZ.data_ptr(),
+             ldz if dZ is None else _ld(dZ, "dZ", m, n, dtype), _stream(stream, Z)))
 
 
-def _matrices(t, what: str, groups: int, rows: int, cols: int) -> tuple[int, int]:
-    """Checks a (groups, rows, cols) CUDA tensor; its leading dimension and
-    the distance between matrices."""
-    _require(t.is_cuda and t.dim() == 3 and tuple(t.shape) == (groups, rows, cols),
-             f"{what}: {tuple(t.shape)} where {(groups, rows, cols)} is wanted")
-    _require(t.stride(2) == 1 or cols <= 1, f"{what}: rows have to be contiguous")
-    ld = int(t.stride(1)) if rows > 1 else max(int(t.stride(1)), cols)
-    return ld, int(t.stride(0))
+def _stacked(t, what: str, groups: int, rows: int, cols: int) -> tuple[int, int]:
+    """The leading dimension and the distance of (groups, rows, cols) matrices."""
+    if t.shape != (groups, rows, cols) or not t.is_cuda:
+        raise PfError(1, f"{what}: a CUDA tensor of {(groups, rows, cols)} is wanted, not of "
+                         f"{tuple(t.shape)} on {t.device}")
+    plane, ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise PfError(1, f"{what}: rows have to be contiguous")
+    return (ld if rows > 1 else max(ld, cols)), plane
 
 
 def grouped_mm(handle: Handle, group_ptr, X, W, Y, transpose_w: bool = True, alpha: float = 1.0,
@@ -382,19 +406,19 @@ def grouped_mm(handle: Handle, group_ptr, X, W, Y, transpose_w: bool = True, alp
     group_ptr[g] <= r < group_ptr[g+1] (CUDA tensors; X rows x k and Y rows x n
     of one 16-bit type). transpose_w: W is (groups, n, k) and op transposes it
     (a layer's forward); otherwise W is (groups, k, n) (the gradient of the
-    layer's input, with dY for X). Group sizes are not read back to the host."""
-    _index(group_ptr, "group_ptr", 1)
+    layer's input, with dY for X). W may be one matrix expanded to all groups.
+    Group sizes are not read back to the host."""
+    dtype = X.dtype
+    f = _entry("gmm", dtype, group_ptr.dtype)
     groups = group_ptr.shape[0] - 1
-    _require(X.dim() == 2 and Y.dim() == 2, "X, Y: 2-d tensors are wanted")
-    rows, k, n = X.shape[0], X.shape[1], Y.shape[1]
-    _require(X.element_size() == 2 and X.is_floating_point() and W.dtype == X.dtype,
-             "X, W, Y: one 16-bit type is wanted")
-    ldx, ldy = _rowmajor(X, "X", rows, k, X.dtype), _rowmajor(Y, "Y", rows, n, X.dtype)
-    ldw, stride_w = _matrices(W, "W", groups, *((n, k) if transpose_w else (k, n)))
-    f = getattr(lib, "pf_gmm_" + _suffix(2, group_ptr.element_size(), X.dtype))
-    _check(f(handle.ptr, groups, rows, n, k, group_ptr.data_ptr(), X.data_ptr(), ldx,
-             W.data_ptr(), ldw, stride_w, int(transpose_w), alpha, beta, Y.data_ptr(), ldy,
-             _stream(stream)))
+    rows, k, n = X.shape[0], X.shape[-1], Y.shape[-1]
+    ldx, ldy = _ld(X, "X", rows, k, dtype), _ld(Y, "Y", rows, n, dtype)
+    ldw, plane = _stacked(W, "W", groups, n, k) if transpose_w else _stacked(W, "W", groups, k, n)
+    if W.dtype != dtype:
+        raise PfError(1, f"W: {W.dtype} where X is of {dtype}")
+    _check(f(handle.ptr, groups, rows, n, k, _flat(group_ptr, "group_ptr", 1, group_ptr.dtype),
+             X.data_ptr(), ldx, W.data_ptr(), ldw, plane, transpose_w, alpha, beta, Y.data_ptr(),
+             ldy, _stream(stream, X)))
 
 
 def grouped_wgrad(handle: Handle, group_ptr, dY, X, dW, alpha: float = 1.0, beta: float = 0.0,
@@ -402,19 +426,17 @@ def grouped_wgrad(handle: Handle, group_ptr, dY, X, dW, alpha: float = 1.0, beta
     """dW[g] = alpha * dY_g^T X_g + beta*dW[g] over the rows of every group g
     (CUDA tensors; dY rows x n and X rows x k of one 16-bit type, dW (groups, n,
     k) of that type or float32): the gradient of the W of ``grouped_mm``."""
-    _index(group_ptr, "group_ptr", 1)
+    dtype = X.dtype
+    f = _entry("gmm_wgrad", dtype, group_ptr.dtype)
     groups = group_ptr.shape[0] - 1
-    _require(X.dim() == 2 and dY.dim() == 2, "dY, X: 2-d tensors are wanted")
-    rows, k, n = X.shape[0], X.shape[1], dY.shape[1]
-    _require(X.element_size() == 2 and X.is_floating_point() and
-             (dW.dtype == X.dtype or str(dW.dtype) == "torch.float32"),
-             "dY, X: one 16-bit type is wanted, dW: that or float32")
-    ldx, lddy = _rowmajor(X, "X", rows, k, X.dtype), _rowmajor(dY, "dY", rows, n, X.dtype)
-    lddw, stride_dw = _matrices(dW, "dW", groups, n, k)
-    f = getattr(lib, "pf_gmm_wgrad_" + _suffix(2, group_ptr.element_size(), X.dtype))
-    _check(f(handle.ptr, groups, rows, n, k, group_ptr.data_ptr(), dY.data_ptr(), lddy,
-             X.data_ptr(), ldx, alpha, beta, dW.data_ptr(), dW.element_size(), lddw, stride_dw,
-             _stream(stream)))
+    rows, k, n = X.shape[0], X.shape[-1], dY.shape[-1]
+    ldx, lddy = _ld(X, "X", rows, k, dtype), _ld(dY, "dY", rows, n, dtype)
+    lddw, plane = _stacked(dW, "dW", groups, n, k)
+    if dW.dtype != dtype and dW.dtype != _F32:
+        raise PfError(1, f"dW: {dW.dtype} where {dtype} or torch.float32 is wanted")
+    _check(f(handle.ptr, groups, rows, n, k, _flat(group_ptr, "group_ptr", 1, group_ptr.dtype),
+             dY.data_ptr(), lddy, X.data_ptr(), ldx, alpha, beta, dW.data_ptr(),
+             dW.element_size(), lddw, plane, _stream(stream, X)))
 
 
 def spmv_dist(handle: Handle, m: int, n: int, nnz: int, row_ptr, col, val, x, prev_slots,

@@ -6,6 +6,48 @@
 
 namespace pf {
 
+template <typename VT, typename IT, int NT, bool GRAD, bool LOOP>
+static pf_status launch_kernel(DistillParams<VT, IT> p, int C, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  // a grid holds less than 2^31 CTAs
+  const int64_t most = (int64_t)1 << 27;
+  for (int64_t r = 0, m = p.m; r < m; r += most) {
+    p.m = std::min(most, m - r);
+    cfg.gridDim = dim3((unsigned)(p.m * C));
+    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_kernel<VT, IT, NT, GRAD, LOOP>, p));
+    count_launches(1);
+    p.row_ptr += p.m;
+    p.Z += p.m * p.ldz;
+    if (p.dZ) p.dZ += p.m * p.lddz;
+    if (p.weight) p.weight += p.m;
+    if (p.loss) p.loss += p.m;
+  }
+  return PF_OK;
+}
+
+// CTAs a row and threads a CTA: the smallest that hold the row in registers.
+// Few rows are spread over more, smaller CTAs, until they fill the GPU.
+template <typename VT, typename IT, bool GRAD>
+static pf_status launch_rows(pf_handle h, const DistillParams<VT, IT> &p, cudaStream_t st) {
+  const int64_t need = p.n + 16 / (int)sizeof(VT) - 1;  // and the alignment's elements
+  int C = 1;
+  while (C < 8 && need > (int64_t)C * 512 * DISTILL_EPT) C *= 2;
+  while (C < 8 && p.m * C * 2 <= h->num_sms && need > (int64_t)C * 128 * DISTILL_EPT) C *= 2;
+  const int64_t each = ceil_div(need, C);
+  if (each <= 128 * DISTILL_EPT) return launch_kernel<VT, IT, 128, GRAD, false>(p, C, st);
+  if (each <= 256 * DISTILL_EPT) return launch_kernel<VT, IT, 256, GRAD, false>(p, C, st);
+  if (each <= 512 * DISTILL_EPT) return launch_kernel<VT, IT, 512, GRAD, false>(p, C, st);
+  return launch_kernel<VT, IT, 512, GRAD, true>(p, C, st);
+}
+
 template <typename VT, typename IT>
 static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, const IT *row_ptr,
                                 const int32_t *col, const VT *val, double temperature, const VT *Z,
@@ -17,7 +59,7 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   PF_CHECK_ARG(temperature > 0.0 && temperature <= 1e30 && temperature >= 1e-30,
                "temperature %g outside [1e-30, 1e30]", temperature);
   if (m == 0) return PF_OK;
-  PF_CHECK_ARG(n <= (int64_t)INT32_MAX, "n must fit int32 column indices");
+  PF_CHECK_ARG(n <= (int64_t)INT32_MAX - 16, "n must be at most 2^31 - 17");
   PF_CHECK_ARG(loss || dZ, "neither loss nor dZ is asked for");
   PF_CHECK_ARG(row_ptr, "null row_ptr");
   PF_CHECK_ARG(nnz == 0 || (col && val), "null col/val with nnz > 0");
@@ -40,7 +82,7 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   p.m = m;
   p.n = n;
   p.nnz = nnz;
-  p.row_ptr = row_ptr;
+  p.row_ptr = p.row_ptr0 = row_ptr;
   p.col = col;
   p.val = val;
   p.Z = Z;
@@ -51,11 +93,7 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   p.lddz = lddz;
   p.inv_tau = (float)(1.0 / temperature);
   p.err = h->err;
-  const unsigned grid = (unsigned)std::min<int64_t>(m, INT32_MAX);
-  distill_kernel<VT, IT, 512><<<grid, 512, 0, st>>>(p);
-  count_launches(1);
-  PF_CUDA_TRY(cudaGetLastError());
-  return PF_OK;
+  return dZ ? launch_rows<VT, IT, true>(h, p, st) : launch_rows<VT, IT, false>(h, p, st);
 }
 
 }  // namespace pf

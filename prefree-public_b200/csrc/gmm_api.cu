@@ -127,14 +127,10 @@ static pf_status wgrad_tc(pf_handle h, const VT *dY, int64_t lddy, const VT *X, 
                           const GmmTcParams<IT, OT> &p, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<VT, __nv_bfloat16>::value;
   GmmMaps maps = {};
-  CUtensorMap *m[3][2] = {{&maps.a, &maps.b}, {&maps.a8, &maps.b8}, {&maps.a1, &maps.b1}};
-  const int box[3] = {64, 8, 1};
-  for (int i = 0; i < 3; ++i) {
-    pf_status s = encode(m[i][0], X, p.ni, p.rows, ldx, 0, 0, box[i]);
-    if (s != PF_OK) return s;
-    s = encode(m[i][1], dY, p.nj, p.rows, lddy, 0, 0, box[i]);
-    if (s != PF_OK) return s;
-  }
+  pf_status s = encode(&maps.a, X, p.ni, p.rows, ldx, 0, 0, 64);
+  if (s != PF_OK) return s;
+  s = encode(&maps.b, dY, p.nj, p.rows, lddy, 0, 0, 64);
+  if (s != PF_OK) return s;
   if (p.ni > 128 && p.nj > 128) return launch_tc<GMM_DW, 2, 256, BF16>(h, maps, p, st);
   return launch_tc<GMM_DW, 1, 128, BF16>(h, maps, p, st);
 }

@@ -37,15 +37,18 @@ struct GroupWalk {
   int64_t before = 0;  // items of the groups before it
   int64_t first = 0;   // group g's first row and number of rows
   int64_t count = 0;
+  int64_t items = 0;   // its items, where they are known
 
   // finds item t; false when there are fewer. Afterwards group g holds it, at
   // place t - before.
   __device__ __forceinline__ bool seek(int64_t t, int tile_rows, int64_t per) {
     const int lane = threadIdx.x & 31;
+    if (t < before + items) return true;
     while (g < groups) {
       int64_t f = 0, c = 0;
       if (g + lane < groups) c = group_rows(ptr, g + lane, rows, &f, err);
-      int64_t sum = (c + tile_rows - 1) / tile_rows * per;
+      const int64_t own = (c + tile_rows - 1) / tile_rows * per;
+      int64_t sum = own;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t v = __shfl_up_sync(~0u, sum, d);
@@ -59,9 +62,11 @@ struct GroupWalk {
         g += k;
         first = __shfl_sync(~0u, f, k);
         count = __shfl_sync(~0u, c, k);
+        items = __shfl_sync(~0u, own, k);
         return true;
       }
       before += __shfl_sync(~0u, sum, 31);
+      items = 0;
       g += 32;
     }
     return false;

@@ -19,9 +19,11 @@
 // itself.
 //
 // DW: rows past a group's end belong to the next group and must not meet the
-// sum (0 * NaN is NaN). The group's last block is copied in boxes of 8 rows
-// and single rows, and filled up to a multiple of 16 by boxes that lie wholly
-// outside of the array, which TMA fills with zeros.
+// sum (0 * NaN is NaN). A group's last, partial block is announced to a warp of
+// its own, which clears the rows up to the next multiple of 16 (what the matrix
+// instruction reads) in both operands before it passes the stage on. (Copying
+// the tail in boxes of 8 rows and single rows instead, filled up by boxes
+// outside of the array, cost 3 us a tile.)
 #pragma once
 
 #include "gmm_common.cuh"
@@ -32,9 +34,7 @@ namespace pf {
 enum GmmMode { GMM_FWD = 0, GMM_DX = 1, GMM_DW = 2 };
 
 struct GmmMaps {
-  CUtensorMap a, b;       // boxes of 64 along p (DW: 64 rows)
-  CUtensorMap a8, b8;     // DW: boxes of 8 rows
-  CUtensorMap a1, b1;     // DW: single rows
+  CUtensorMap a, b;
 };
 
 template <typename IT, typename OT>
@@ -58,7 +58,7 @@ struct GmmTcParams {
 // to a line keep the banks apart. Storing straight from the registers, 2 bytes
 // a lane and 64 bytes an instruction, bound the kernel: 790 us against 82 us of
 // DRAM time for 64 gradients of 2048 x 2048.
-constexpr int GMM_STAGING = 32 * (128 + 16);
+constexpr int GMM_STAGING = 64 * (64 + 16);  // and 32 * (128 + 16) is less
 
 template <typename OT>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -75,48 +75,50 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
 template <>
 __device__ __forceinline__ uint32_t pack2<float>(float, float) { return 0; }  // not called
 
-// 32 lanes x 32 columns of tensor memory -> alpha * v, rounded, [column][lane]
+// 32 lanes x 64 columns of tensor memory -> alpha * v, rounded, [column][lane]
+// in two areas of 32 columns, 32 * 80 bytes each
 template <typename OT>
 __device__ __forceinline__ void stage_pairs(uint8_t *stage, uint32_t src, float alpha) {
   const int lane = threadIdx.x & 31;
-  float lo[16], hi[16];  // lanes 0-15 and 16-31: fragments of 8 x 8
-  tc::tmem_load16x256b_x4(src, lo);
-  tc::tmem_load16x256b_x4(src + (16u << 16), hi);
+  float v[4][16];  // lanes 0-15 and 16-31 of two times 32 columns: fragments of 8 x 8
+  tc::tmem_load16x256b_x4(src, v[0]);
+  tc::tmem_load16x256b_x4(src + (16u << 16), v[1]);
+  tc::tmem_load16x256b_x4(src + 32, v[2]);
+  tc::tmem_load16x256b_x4(src + 32 + (16u << 16), v[3]);
   tc::tmem_load_wait();
   const uint32_t at = ptx::smem_addr(stage) + (lane & 7) * 80 + (lane >> 3) * 16;
 #pragma unroll
-  for (int b = 0; b < 4; ++b)  // eight columns
-    tc::store_matrices_t(at + b * 8 * 80,
-                         pack2<OT>(alpha * lo[4 * b], alpha * lo[4 * b + 1]),
-                         pack2<OT>(alpha * lo[4 * b + 2], alpha * lo[4 * b + 3]),
-                         pack2<OT>(alpha * hi[4 * b], alpha * hi[4 * b + 1]),
-                         pack2<OT>(alpha * hi[4 * b + 2], alpha * hi[4 * b + 3]));
+  for (int b = 0; b < 8; ++b) {  // eight columns
+    const float *lo = v[b / 4 * 2] + b % 4 * 4, *hi = v[b / 4 * 2 + 1] + b % 4 * 4;
+    tc::store_matrices_t(at + b * 8 * 80, pack2<OT>(alpha * lo[0], alpha * lo[1]),
+                         pack2<OT>(alpha * lo[2], alpha * lo[3]),
+                         pack2<OT>(alpha * hi[0], alpha * hi[1]),
+                         pack2<OT>(alpha * hi[2], alpha * hi[3]));
+  }
 }
-// C's rows are 16-byte aligned; ni of 32 i and nj of 32 j exist
+// C's rows are 16-byte aligned; ni of 32 i and nj of 64 j exist
 template <typename OT>
 __device__ __forceinline__ void store_pairs(const uint8_t *stage, OT *c, int64_t ldc, int ni,
                                             int nj) {
   const int lane = threadIdx.x & 31, x = lane & 3;
-  if (ni == 32 && nj == 32) {
-    const uint8_t *from = stage + (lane >> 2) * 80 + x * 16;
-    OT *p = c + (lane >> 2) * ldc + x * 8;
-    uint4 v[4];
+  const uint8_t *from = stage + (lane >> 2) * 80 + x * 16;
+  OT *p = c + (lane >> 2) * ldc + x * 8;
+  if (ni == 32 && nj == 64) {
+    uint4 v[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = *reinterpret_cast<const uint4 *>(from + q * 640);
+    for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const uint4 *>(from + q * 640);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4 *>(p + q * 8 * ldc) = v[q];
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4 *>(p + q * 8 * ldc) = v[q];
     return;
   }
 #pragma unroll 1
-  for (int q = 0; q < 4; ++q) {
-    const int j = q * 8 + (lane >> 2);
-    if (j >= nj) continue;
-    const uint4 v = *reinterpret_cast<const uint4 *>(stage + j * 80 + x * 16);
-    OT *p = c + j * ldc + x * 8;
+  for (int j = lane >> 2; j < nj; j += 8, from += 640, p += 8 * ldc) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(from);
     if (x * 8 + 8 <= ni) {
       *reinterpret_cast<uint4 *>(p) = v;
     } else {
-      const OT *e = reinterpret_cast<const OT *>(&v);
+      alignas(16) OT e[8];
+      *reinterpret_cast<uint4 *>(e) = v;
       for (int y = 0; y < ni - x * 8; ++y) p[y] = e[y];
     }
   }
@@ -180,11 +182,17 @@ struct GmmCfg {
   static constexpr int STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 200 * 1024 / STAGE > 10 ? 10 : 200 * 1024 / STAGE;
   static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;  // tensor memory columns
-  static constexpr int NT = 192;
+  static constexpr int NT = MODE == GMM_DW ? 224 : 192;
   static constexpr int SMEM = STAGES * STAGE + 4 * GMM_STAGING + 1024;  // and alignment
 };
 
 constexpr uint64_t GMM_WAIT_NS = 4000000000ull;
+
+// columns that the matrix instruction computes for jn outputs
+template <int CG>
+__device__ __forceinline__ int instr_cols(int jn) {
+  return (jn + 16 * CG - 1) / (16 * CG) * (16 * CG);
+}
 
 // One tile: where it lies and how long its sum is.
 struct GmmTile {
@@ -203,30 +211,47 @@ struct GmmTiles {
   GroupWalk<IT> walk;
   int ti, tj;
   int64_t t, step;
+  int64_t g = 0;           // DW: the next tile's group and place in it
+  int l = 0, step_l = 0;
+  int64_t step_g = 0;
 
   __device__ GmmTiles(const GmmTcParams<IT, OT> &p)
       : P(p), walk{p.ptr, p.groups, p.rows, p.err}, ti((p.ni + Cfg::TI - 1) / Cfg::TI),
-        tj(MODE == GMM_DW ? (p.nj + BN - 1) / BN : 0), t(blockIdx.x / CG), step(gridDim.x / CG) {}
+        tj(MODE == GMM_DW ? (p.nj + BN - 1) / BN : 0), t(blockIdx.x / CG), step(gridDim.x / CG) {
+    if constexpr (MODE == GMM_DW) {
+      const int64_t per = (int64_t)ti * tj;
+      g = t / per;
+      l = (int)(t - g * per);
+      step_g = step / per;
+      step_l = (int)(step - step_g * per);
+    }
+  }
 
   // the next tile of this CTA (all lanes of a warp together)
   __device__ __forceinline__ bool next(GmmTile *o) {
     if constexpr (MODE == GMM_DW) {
-      const int64_t per = (int64_t)ti * tj;
-      o->g = t / per;
-      if (o->g >= P.groups) return false;
-      const int l = (int)(t - o->g * per);
+      if (g >= P.groups) return false;
+      o->g = g;
       o->np = (int)group_rows(P.ptr, o->g, P.rows, &o->p0, P.err);
       o->i0 = l % ti * Cfg::TI;
       o->j0 = (int64_t)(l / ti) * BN;
       o->jn = min(BN, P.nj - (int)o->j0);
+      g += step_g;
+      l += step_l;
+      if (l >= ti * tj) l -= ti * tj, ++g;
     } else {
       if (!walk.seek(t, BN, ti)) return false;
+      // rows and n fit 31 bits, and so do a group's row tiles; its tiles may not
       const int64_t l = t - walk.before;
-      const int64_t jt = l / ti;
+      const int jt = l <= INT32_MAX ? (int)l / ti : (int)(l / ti);
       o->g = walk.g;
-      o->i0 = (int)(l - jt * ti) * Cfg::TI;
-      o->j0 = walk.first + jt * BN;
-      o->jn = (int)min((int64_t)BN, walk.count - jt * BN);
+      o->i0 = (int)(l - (int64_t)jt * ti) * Cfg::TI;
+      // the group's tiles are of equal size, up to the instruction's step: full
+      // ones and a remainder would leave some CTAs with more to do than others
+      const int nt = (int)((walk.count + BN - 1) / BN);
+      const int each = instr_cols<CG>((int)((walk.count + nt - 1) / nt));
+      o->j0 = walk.first + (int64_t)jt * each;
+      o->jn = (int)min((int64_t)each, walk.count - (int64_t)jt * each);
       o->np = P.np;
       o->p0 = 0;
     }
@@ -235,33 +260,13 @@ struct GmmTiles {
   }
 };
 
-// A panel of `valid` < 64 rows from `row` on, filled up to a multiple of 16 with
-// zero rows (boxes at row `outside`, past the array).
-template <int CG>
-__device__ __forceinline__ void load_ragged(uint32_t dst, const CUtensorMap *m8,
-                                            const CUtensorMap *m1, uint32_t bar, int c, int row,
-                                            int valid, int outside) {
-  for (int r = 0; r < (valid + 15) / 16 * 16; r += 8) {
-    if (r + 8 <= valid || r >= valid)
-      tc::load_2d<CG>(dst + r * 128, m8, bar, c, r < valid ? row + r : outside);
-    else
-      for (int q = r; q < r + 8; ++q)
-        tc::load_2d<CG>(dst + q * 128, m1, bar, c, q < valid ? row + q : outside);
-  }
-}
-
-// columns that the matrix instruction computes for jn outputs
-template <int CG>
-__device__ __forceinline__ int instr_cols(int jn) {
-  return (jn + 16 * CG - 1) / (16 * CG) * (16 * CG);
-}
-
 template <int MODE, int CG, int BN, bool BF16, typename IT, typename OT>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(GmmCfg<MODE, CG, BN>::NT, 1)
 gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   using Cfg = GmmCfg<MODE, CG, BN>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[Cfg::STAGES], empty[Cfg::STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint64_t tail[Cfg::STAGES];  // DW
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -271,8 +276,9 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   if (tid == 0) {
     dead = 0;
     for (int s = 0; s < Cfg::STAGES; ++s) {
-      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&full[s], CG);
       ptx::mbar_init(&empty[s], 1);
+      ptx::mbar_init(&tail[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&acc_full[s], 1);
@@ -319,31 +325,28 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
           const uint32_t sa = stage0 + s * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
           const uint32_t bar = full_at + s * 8;
           if constexpr (MODE == GMM_DW) {
-            const int left = t.np - kb * 64;
-            const int valid = left < 64 ? left : 64, r16 = (valid + 15) / 16 * 16;
             const int panels_b = (half + 63) / 64;
-            if (rank == 0)
-              ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)(CG * (2 + panels_b) * r16 * 128));
-            const int row = (int)t.p0 + kb * 64;
-            const int jb = (int)t.j0 + (int)rank * half;
-            if (valid == 64) {
-              tc::load_2d<CG>(sa, &M.a, bar, ia, row);
-              tc::load_2d<CG>(sa + 8192, &M.a, bar, ia + 64, row);
-              for (int x = 0; x < panels_b; ++x)
-                tc::load_2d<CG>(sb + x * 8192, &M.b, bar, jb + x * 64, row);
-            } else {
-              for (int x = 0; x < 2; ++x)
-                load_ragged<CG>(sa + x * 8192, &M.a8, &M.a1, bar, ia + x * 64, row, valid,
-                                (int)P.rows);
-              for (int x = 0; x < panels_b; ++x)
-                load_ragged<CG>(sb + x * 8192, &M.b8, &M.b1, bar, jb + x * 64, row, valid,
-                                (int)P.rows);
+            const uint32_t bytes = (uint32_t)(2 + panels_b) * 8192;
+            const bool whole = t.np - kb * 64 >= 64;
+            const uint32_t to = whole ? bar : tc::smem_addr(&tail[s]);
+            if (!whole) {
+              ptx::mbar_arrive_expect_tx(&tail[s], bytes);
+            } else if (rank == 0) {
+              ptx::mbar_arrive_expect_tx(&full[s], CG * bytes);
+              if (CG == 2) ptx::mbar_arrive(&full[s]);
             }
+            const int row = (int)t.p0 + kb * 64, jb = (int)t.j0 + (int)rank * half;
+            tc::load_2d<CG>(sa, &M.a, to, ia, row);
+            tc::load_2d<CG>(sa + 8192, &M.a, to, ia + 64, row);
+            for (int x = 0; x < panels_b; ++x)
+              tc::load_2d<CG>(sb + x * 8192, &M.b, to, jb + x * 64, row);
           } else {
             const int boxes = (half + Cfg::BOX - 1) / Cfg::BOX;
-            if (rank == 0)
+            if (rank == 0) {
               ptx::mbar_arrive_expect_tx(
                   &full[s], (uint32_t)(CG * (Cfg::A_BYTES + boxes * Cfg::BOX * 128)));
+              if (CG == 2) ptx::mbar_arrive(&full[s]);
+            }
             if constexpr (MODE == GMM_FWD) {
               tc::load_3d<CG>(sa, &M.a, bar, kb * 64, ia, gw);
             } else {
@@ -380,6 +383,9 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
           ok = false;
           break;
         }
+        // the other CTA's cleared rows (a wait of this scope at every block costs
+        // as much as two blocks)
+        if (CG == 2 && MODE == GMM_DW && t.np - kb * 64 < 64) tc::acquire_cluster(&full[s], ph);
         tc::fence_after_sync();
         if (tc::elect()) {
           const uint32_t sa = stage0 + s * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
@@ -396,6 +402,30 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
         }
         __syncwarp();
       }
+    }
+  } else if (MODE == GMM_DW && wid == 6) {  // ---- rows past a group's end
+    const uint32_t full_at = CG == 2 ? tc::map_rank(tc::smem_addr(&full[0]), 0)
+                                     : tc::smem_addr(&full[0]);
+    uint32_t it = 0, parity = 0;  // parity: one bit to a stage, flipped at each use
+    while (tiles.next(&t)) {
+      const int nb = (t.np + 63) / 64, valid = t.np & 63;
+      it += nb;
+      if (valid == 0) continue;
+      const uint32_t s = (it - 1) % Cfg::STAGES;
+      if (!wait(&tail[s], parity >> s & 1)) break;
+      parity ^= 1u << s;
+      const int panels = 2 + (instr_cols<CG>(t.jn) / CG + 63) / 64;
+      const int zero = ((valid + 15) & ~15) - valid;  // the matrix instruction reads no more
+      uint8_t *at = raw + (stage0 - tc::smem_addr(raw)) + s * Cfg::STAGE + valid * 128;
+      for (int x = lane; x < panels * zero * 8; x += 32) {
+        const int p = x / (zero * 8);
+        *reinterpret_cast<uint4 *>(at + p * 8192 + (x - p * zero * 8) * 16) =
+            make_uint4(0, 0, 0, 0);
+      }
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_release(full_at + s * 8);
+      __syncwarp();
     }
   } else if (wid >= 2) {  // ---- accumulator to C
     const int quad = wid & 3;  // the tensor memory lanes that this warp may read
@@ -415,22 +445,32 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       const int i0 = t.i0 + (int)rank * 128 + quad * 32;  // this warp's 32 of i
       OT *c = P.C + (MODE == GMM_DW ? t.g * P.stride_c : 0) + t.j0 * P.ldc + i0;
       const uint32_t src = tmem + ((uint32_t)quad << 21) + buf * BN;
-      for (int j = 0; j < t.jn; j += 32, c += 32 * P.ldc) {
-        const bool last = j + 32 >= t.jn;
-        if (sizeof(OT) == 2 && sum && P.plain)
-          stage_pairs<OT>(stage, src + j, P.alpha);
-        else
-          stage_floats(stage, src + j, sum);
+      // the accumulator has been read: hand it back
+      auto release = [&] {
         tc::fence_before_sync();
         __syncwarp();
-        if (sum && last && lane == 0) {  // the accumulator has been read: free it
+        if (lane == 0) {
           if (CG == 2) tc::mbar_arrive_cluster(tc::map_rank(tc::smem_addr(&acc_empty[buf]), 0));
           else ptx::mbar_arrive(&acc_empty[buf]);
         }
-        const int nj = min(32, t.jn - j), ni = min(32, P.ni - i0);
-        if (sizeof(OT) == 2 && sum && P.plain) store_pairs(stage, c, P.ldc, ni, nj);
-        else store_floats(stage, c, P.ldc, ni, nj, P.alpha, P.beta, P.aligned);
-        __syncwarp();
+      };
+      const int ni = min(32, P.ni - i0);
+      if (BN >= 64 && sizeof(OT) == 2 && sum && P.plain) {
+        for (int j = 0; j < t.jn; j += 64, c += 64 * P.ldc) {
+          stage_pairs<OT>(stage, src + j, P.alpha);
+          if (j + 64 >= t.jn) release();
+          else __syncwarp();
+          store_pairs(stage, c, P.ldc, ni, min(64, t.jn - j));
+          __syncwarp();
+        }
+      } else {
+        for (int j = 0; j < t.jn; j += 32, c += 32 * P.ldc) {
+          stage_floats(stage, src + j, sum);
+          if (sum && j + 32 >= t.jn) release();
+          else __syncwarp();
+          store_floats(stage, c, P.ldc, ni, min(32, t.jn - j), P.alpha, P.beta, P.aligned);
+          __syncwarp();
+        }
       }
     }
   }

@@ -46,6 +46,25 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
                : "memory");
 }
 
+// with release (this thread's and, after a barrier, its warp's writes), for a
+// waiter in another CTA of the cluster that calls acquire_cluster
+__device__ __forceinline__ void mbar_arrive_release(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+// after a wait for this phase has succeeded: acquires what arrivals of other
+// CTAs released
+__device__ __forceinline__ void acquire_cluster(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
