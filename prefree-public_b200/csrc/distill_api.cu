@@ -6,10 +6,16 @@
 
 namespace pf {
 
-template <typename VT, typename IT, int NT, bool GRAD, bool LOOP>
-static pf_status launch_kernel(DistillParams<VT, IT> p, int C, cudaStream_t st) {
+constexpr int kMaxDevices = 64;
+
+template <typename VT, typename IT, int NT, bool GRAD>
+static pf_status launch_kernel(pf_handle h, const DistillParams<VT, IT> &p, int C,
+                               cudaStream_t st) {
+  using Cfg = DistillCfg<VT, NT>;
+  auto kern = distill_kernel<VT, IT, NT, GRAD>;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(NT);
+  cfg.blockDim = dim3(NT + 64);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -17,35 +23,40 @@ static pf_status launch_kernel(DistillParams<VT, IT> p, int C, cudaStream_t st) 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  // a grid holds less than 2^31 CTAs
-  const int64_t most = (int64_t)1 << 27;
-  for (int64_t r = 0, m = p.m; r < m; r += most) {
-    p.m = std::min(most, m - r);
-    cfg.gridDim = dim3((unsigned)(p.m * C));
-    PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_kernel<VT, IT, NT, GRAD, LOOP>, p));
-    count_launches(1);
-    p.row_ptr += p.m;
-    p.Z += p.m * p.ldz;
-    if (p.dZ) p.dZ += p.m * p.lddz;
-    if (p.weight) p.weight += p.m;
-    if (p.loss) p.loss += p.m;
+  // clusters that the device holds at once, per device and size (0 = not yet)
+  static int held[kMaxDevices][DISTILL_MAX_C + 1] = {};
+  int &most = held[h->device % kMaxDevices][C];
+  if (most == 0) {
+    PF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    cfg.gridDim = dim3(C);
+    int v = 0;
+    PF_CUDA_TRY(cudaOccupancyMaxActiveClusters(&v, kern, &cfg));
+    most = std::max(1, v);
   }
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.m, most) * C));
+  PF_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
+  count_launches(1);
   return PF_OK;
 }
 
-// CTAs a row and threads a CTA: the smallest that hold the row in registers.
-// Few rows are spread over more, smaller CTAs, until they fill the GPU.
+// CTAs a row and threads a CTA. One CTA a row, of the fewest threads that take
+// it at once; few rows are spread over more CTAs, until they fill the GPU, and
+// so are rows whose gradient is to find them in L2 (kRowsInHand bytes at most
+// in hand on the whole GPU).
+constexpr int64_t kRowsInHand = 40 << 20;
+
 template <typename VT, typename IT, bool GRAD>
 static pf_status launch_rows(pf_handle h, const DistillParams<VT, IT> &p, cudaStream_t st) {
-  const int64_t need = p.n + 16 / (int)sizeof(VT) - 1;  // and the alignment's elements
+  constexpr int64_t SMALL = DistillCfg<VT, 64>::PIECE;
+  const int64_t need = ceil_div(p.n, DistillCfg<VT, 64>::VE) + 1;  // pieces
   int C = 1;
-  while (C < 8 && need > (int64_t)C * 512 * DISTILL_EPT) C *= 2;
-  while (C < 8 && p.m * C * 2 <= h->num_sms && need > (int64_t)C * 128 * DISTILL_EPT) C *= 2;
-  const int64_t each = ceil_div(need, C);
-  if (each <= 128 * DISTILL_EPT) return launch_kernel<VT, IT, 128, GRAD, false>(p, C, st);
-  if (each <= 256 * DISTILL_EPT) return launch_kernel<VT, IT, 256, GRAD, false>(p, C, st);
-  if (each <= 512 * DISTILL_EPT) return launch_kernel<VT, IT, 512, GRAD, false>(p, C, st);
-  return launch_kernel<VT, IT, 512, GRAD, true>(p, C, st);
+  while (GRAD && C < DISTILL_MAX_C && need > C * 4 * SMALL &&
+         need * 16 * (2 * h->num_sms / C) > kRowsInHand)
+    C *= 2;
+  while (C < DISTILL_MAX_C && p.m * C * 2 <= h->num_sms && need > C * SMALL) C *= 2;
+  if (need <= C * SMALL) return launch_kernel<VT, IT, 64, GRAD>(h, p, C, st);
+  if (need <= C * 2 * SMALL) return launch_kernel<VT, IT, 128, GRAD>(h, p, C, st);
+  return launch_kernel<VT, IT, 256, GRAD>(h, p, C, st);
 }
 
 template <typename VT, typename IT>
