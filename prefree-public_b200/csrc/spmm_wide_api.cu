@@ -29,6 +29,12 @@ static pf_status check_wide(pf_handle h, int64_t m, int64_t n, int64_t nnz, cons
   return PF_OK;
 }
 
+// whether every row starts on a 16-byte boundary
+template <typename VT>
+static bool rows16(const VT *p, int64_t ld) {
+  return ((uintptr_t)p % 16) == 0 && ld % 8 == 0;
+}
+
 template <typename VT, typename IT>
 static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, const IT *row_ptr,
                                const int32_t *col, const VT *val, int k, double alpha, const VT *X,
@@ -40,8 +46,23 @@ static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, c
   if (s != PF_OK) return s;
   WideParams<VT, IT> p{m, n, nnz, row_ptr, col, val, X, ldx, Y, ldy, nullptr, k,
                        (float)alpha, (float)beta, h->err};
-  const unsigned grid = (unsigned)std::min<int64_t>(m, INT32_MAX);
-  spmm_wide_kernel<VT, IT, 256><<<grid, 256, 0, st>>>(p);
+  // rows of one or two non-zeros (a dispatch, or a gradient of the slots) take
+  // several pieces of columns at a time instead of several non-zeros
+  const bool aligned = rows16(X, ldx) && rows16(Y, ldy);
+  const bool few = nnz <= 2 * m;
+  const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? 4 : 1);
+  // threads a row: one for every unit of its columns, up to a CTA; the columns of
+  // few rows are spread over more CTAs
+  int tpr_log2 = 0;
+  while (tpr_log2 < 8 && (1 << tpr_log2) < units) ++tpr_log2;
+  while (tpr_log2 > 5 && ceil_div(m, 256 >> tpr_log2) < h->num_sms) --tpr_log2;
+  const int64_t ctas = ceil_div(m, 256 >> tpr_log2), most = (int64_t)h->num_sms * (aligned ? 4 : 3);
+  dim3 grid((unsigned)std::min(ctas, most));
+  if (ctas < h->num_sms) grid.y = (unsigned)std::min<int64_t>(64, ceil_div(units, 1 << tpr_log2));
+  if (aligned && few) spmm_wide_kernel<VT, IT, 256, true, 1, 4><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else if (aligned) spmm_wide_kernel<VT, IT, 256, true, 4, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else if (few) spmm_wide_kernel<VT, IT, 256, false, 1, 4><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else spmm_wide_kernel<VT, IT, 256, false, 4, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
   count_launches(1);
   PF_CUDA_TRY(cudaGetLastError());
   return PF_OK;
@@ -59,8 +80,14 @@ static pf_status launch_sddmm(pf_handle h, int64_t m, int64_t n, int64_t nnz, co
   if (s != PF_OK) return s;
   WideParams<VT, IT> p{m, n, nnz, row_ptr, col, nullptr, X, ldx, const_cast<VT *>(dY), lddy, dval,
                        k, (float)alpha, (float)beta, h->err};
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(m, 8), INT32_MAX);
-  sddmm_kernel<VT, IT, 256><<<grid, 256, 0, st>>>(p);
+  // warps a row: as many as it has non-zeros on average
+  int wpr_log2 = 0;
+  while (wpr_log2 < 3 && ((int64_t)m << wpr_log2) < nnz) ++wpr_log2;
+  const unsigned grid =
+      (unsigned)std::min<int64_t>(ceil_div(m, 8 >> wpr_log2), (int64_t)h->num_sms * 4);
+  if (rows16(X, ldx) && rows16(dY, lddy))
+    sddmm_kernel<VT, IT, 256, true><<<grid, 256, 0, st>>>(p, wpr_log2);
+  else sddmm_kernel<VT, IT, 256, false><<<grid, 256, 0, st>>>(p, wpr_log2);
   count_launches(1);
   PF_CUDA_TRY(cudaGetLastError());
   return PF_OK;
