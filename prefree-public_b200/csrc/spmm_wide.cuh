@@ -32,8 +32,7 @@ struct WideParams {
 // Dense rows start anywhere. A row is cut into the 16-byte pieces of memory that
 // it lies in; Y's pieces give the columns that a thread holds, and X's columns
 // for one of them lie in two of X's pieces, `d` elements further. The second
-// piece is the neighbour thread's first (a hit in L1), and the shift is the same
-// for a whole row: eight cases with fixed registers. (Elements one by one, or
+// piece is the neighbour thread's first (a hit in L1). (Elements one by one, or
 // pairs in 4-byte words, took 127 and 142 us instead of 33 for the gradients of
 // 3001 tokens of four slots, 1531 columns.) Elements of neighbours are never
 // stored, and masked where they would be summed.
@@ -49,25 +48,16 @@ struct DenseRow {
   }
 };
 
-// elements d .. d + 7 of two pieces
+// elements d .. d + 7 of two pieces: by 4, 2 and 1 elements, in registers
 __device__ __forceinline__ uint4 shifted(const uint4 &a, const uint4 &b, int d) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#define PF_EVEN(i) make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3])
-#define PF_ODD(i)                                                                         \
-  make_uint4(__funnelshift_r(w[i], w[i + 1], 16), __funnelshift_r(w[i + 1], w[i + 2], 16), \
-             __funnelshift_r(w[i + 2], w[i + 3], 16), __funnelshift_r(w[i + 3], w[i + 4], 16))
-  switch (d) {
-    case 0: return PF_EVEN(0);
-    case 1: return PF_ODD(0);
-    case 2: return PF_EVEN(1);
-    case 3: return PF_ODD(1);
-    case 4: return PF_EVEN(2);
-    case 5: return PF_ODD(2);
-    case 6: return PF_EVEN(3);
-    default: return PF_ODD(3);
-  }
-#undef PF_EVEN
-#undef PF_ODD
+  const bool four = (d & 4) != 0, two = (d & 2) != 0;
+  const uint32_t u0 = four ? a.z : a.x, u1 = four ? a.w : a.y, u2 = four ? b.x : a.z,
+                 u3 = four ? b.y : a.w, u4 = four ? b.z : b.x, u5 = four ? b.w : b.y;
+  const uint32_t v0 = two ? u1 : u0, v1 = two ? u2 : u1, v2 = two ? u3 : u2, v3 = two ? u4 : u3,
+                 v4 = two ? u5 : u4;
+  const int by = (d & 1) * 16;
+  return make_uint4(__funnelshift_r(v0, v1, by), __funnelshift_r(v1, v2, by),
+                    __funnelshift_r(v2, v3, by), __funnelshift_r(v3, v4, by));
 }
 
 // The columns of X's row that lie at piece v of a row that starts `shift`
@@ -75,15 +65,15 @@ __device__ __forceinline__ uint4 shifted(const uint4 &a, const uint4 &b, int d) 
 template <typename VT, bool ALIGNED>
 struct Gather {
   uint4 a, b;
-  __device__ __forceinline__ void load(const DenseRow<VT> &x, int v, int shift) {
+  __device__ __forceinline__ void load(const DenseRow<VT> &x, int v, int delta) {
     if (ALIGNED) {
       a = __ldg(x.piece + v);
       return;
     }
-    const int delta = x.shift - shift, p = v + (delta >> 3), d = delta & 7;
+    const int p = v + (delta >> 3);
     a = b = make_uint4(0, 0, 0, 0);
-    if (p >= 0 && p < x.count) a = __ldg(x.piece + p);
-    if (d != 0 && p + 1 < x.count) b = __ldg(x.piece + p + 1);
+    if ((uint32_t)p < (uint32_t)x.count) a = __ldg(x.piece + p);
+    if ((delta & 7) != 0 && p + 1 < x.count) b = __ldg(x.piece + p + 1);
   }
   __device__ __forceinline__ void get(int delta, float (&out)[8]) const {
     unpack<VT>(ALIGNED ? a : shifted(a, b, delta & 7), out);
@@ -94,17 +84,21 @@ struct Gather {
 // not non-decreasing within [row_ptr[0], row_ptr[0] + nnz].
 template <typename VT, typename IT>
 struct RowWalk {
-  const WideParams<VT, IT> &P;
-  int64_t base, s = 0, e = 0;
+  const IT *ptr;
+  int64_t m;
+  IT base, last, s, e;
   __device__ __forceinline__ RowWalk(const WideParams<VT, IT> &p)
-      : P(p), base((int64_t)p.row_ptr[0]) {}
-  __device__ __forceinline__ void fetch(int64_t r) {  // nothing is waited for
-    if (r < P.m) s = (int64_t)P.row_ptr[r], e = (int64_t)P.row_ptr[r + 1];
-    else s = e = base;
+      : ptr(p.row_ptr), m(p.m), base(p.row_ptr[0]) {
+    const int64_t end = (int64_t)base + p.nnz;
+    last = sizeof(IT) == 4 && end > INT32_MAX ? (IT)INT32_MAX : (IT)end;
   }
-  __device__ __forceinline__ void check(bool flag) {
-    if (s < base || e < s || e > base + P.nnz) {
-      if (flag) atomicOr(P.err, PF_DEVERR_ROWPTR);
+  __device__ __forceinline__ void fetch(int64_t r) {  // nothing is waited for
+    s = e = base;
+    if (r < m) s = ptr[r], e = ptr[r + 1];
+  }
+  __device__ __forceinline__ void check(bool flag, unsigned *err) {
+    if (s < base || e < s || e > last) {
+      if (flag) atomicOr(err, PF_DEVERR_ROWPTR);
       s = e = base;
     }
   }
@@ -113,8 +107,9 @@ struct RowWalk {
 // 2^tpr_log2 threads a row, each Q pieces of columns at a time; B non-zeros are
 // gathered before the first is used: 64 bytes on their way to a thread. While a
 // row is worked on, the next one's first columns and values and the bounds of
-// the one after that are fetched: a row costs one latency instead of three
-// (62259 rows of one non-zero, 2048 columns: 109 us without).
+// the one after that are fetched: a row costs one latency instead of three.
+// What bounds it besides DRAM is the number of instructions, so alpha goes into
+// the values, and whole pieces take a path without masks.
 template <typename VT, typename IT, int NT, bool ALIGNED, int B, int Q>
 __global__ void __launch_bounds__(NT, ALIGNED ? 4 : 3)
 spmm_wide_kernel(const WideParams<VT, IT> P, int tpr_log2) {
@@ -123,92 +118,88 @@ spmm_wide_kernel(const WideParams<VT, IT> P, int tpr_log2) {
   const int64_t step = (int64_t)gridDim.x * (NT >> tpr_log2);
   const int64_t r0 = (int64_t)blockIdx.x * (NT >> tpr_log2) + (threadIdx.x >> tpr_log2);
   const bool flag = sub == 0 && blockIdx.y == 0;
+  const uint32_t n = (uint32_t)min(P.n, (int64_t)0xffffffff);
+  const int k = (int)P.k;
   RowWalk<VT, IT> next(P);
   next.fetch(r0);
-  int64_t s = 0, e = 0;
   uint32_t col[B];
   VT val[B];
-  auto entries = [&](int64_t i, int64_t end) {
+  auto entries = [&](IT i, IT end) {
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       col[b] = 0xffffffffu;
-      if (i + b < end) col[b] = (uint32_t)P.col[i + b], val[b] = P.val[i + b];
+      if (end - i > b) col[b] = (uint32_t)P.col[i + b], val[b] = P.val[i + b];
     }
   };
-  next.check(flag && r0 < P.m);
-  s = next.s, e = next.e;
+  next.check(flag && r0 < P.m, P.err);
+  IT s = next.s, e = next.e;
   entries(s, e);
   next.fetch(r0 + step);
   for (int64_t r = r0; r < P.m; r += step) {
     VT *y = P.Y + r * P.ldy;
-    const DenseRow<VT> Y(y, P.k);
-    const int shift = ALIGNED ? 0 : Y.shift;
+    const DenseRow<VT> Y(y, k);
+    const int shift = ALIGNED ? 0 : Y.shift, count = Y.count;
+    // pieces first_whole .. last_whole are all the row's
+    const int first_whole = shift > 0, last_whole = count - 1 - ((k + shift) % 8 != 0);
     bool fetched = true;  // whether col and val are the row's first
-    for (int v = blockIdx.y * tpr * Q + sub; v < Y.count; v += gridDim.y * tpr * Q) {
+    for (int v = blockIdx.y * tpr * Q + sub; v < count; v += gridDim.y * tpr * Q) {
       float acc[Q][8] = {};
-      for (int64_t i = s; i < e; i += B) {
+      for (IT i = s; i < e; i += B) {
         if (!fetched) entries(i, e);
         fetched = false;
         Gather<VT, ALIGNED> x[B][Q];
         int delta[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-          if (col[b] >= (uint64_t)P.n) {
-            if (i + b < e) atomicOr(P.err, PF_DEVERR_BOUNDS);
+          if (col[b] >= n) {
+            if (e - i > b) atomicOr(P.err, PF_DEVERR_BOUNDS);
             col[b] = 0xffffffffu;
             continue;
           }
-          const DenseRow<VT> X(P.X + (int64_t)col[b] * P.ldx, P.k);
-          delta[b] = X.shift - shift;
+          const DenseRow<VT> X(P.X + (int64_t)col[b] * P.ldx, k);
+          delta[b] = ALIGNED ? 0 : X.shift - shift;
 #pragma unroll
           for (int q = 0; q < Q; ++q)
-            if (v + q * tpr < Y.count) x[b][q].load(X, v + q * tpr, shift);
+            if (v + q * tpr < count) x[b][q].load(X, v + q * tpr, delta[b]);
         }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
           if (col[b] == 0xffffffffu) continue;
-          const float a = to_f32(val[b]);
+          const float a = P.alpha * to_f32(val[b]);
 #pragma unroll
-          for (int q = 0; q < Q; ++q)
-            if (v + q * tpr < Y.count) {
-              float f[8];
-              x[b][q].get(delta[b], f);
+          for (int q = 0; q < Q; ++q) {
+            float f[8];
+            x[b][q].get(delta[b], f);  // (past the row: not stored)
 #pragma unroll
-              for (int z = 0; z < 8; ++z) acc[q][z] = fmaf(a, f[z], acc[q][z]);
-            }
+            for (int z = 0; z < 8; ++z) acc[q][z] = fmaf(a, f[z], acc[q][z]);
+          }
         }
       }
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int p = v + q * tpr;
-        if (p >= Y.count) continue;
         VT *to = y - shift + (int64_t)p * 8;
-        const int lo = p == 0 ? shift : 0;
-        const int hi = (int)min((int64_t)8, P.k + shift - (int64_t)p * 8);
-        const bool whole = lo == 0 && hi == 8;
-        if (P.beta != 0.0f) {
-          float old[8] = {};
-          if (whole) unpack<VT>(*reinterpret_cast<const uint4 *>(to), old);
-          else
+        if (p >= first_whole && p <= last_whole) {
+          if (P.beta != 0.0f) {
+            float old[8];
+            unpack<VT>(*reinterpret_cast<const uint4 *>(to), old);
 #pragma unroll
-            for (int z = 0; z < 8; ++z)
-              if (z >= lo && z < hi) old[z] = to_f32(to[z]);
-#pragma unroll
-          for (int z = 0; z < 8; ++z) acc[q][z] = P.alpha * acc[q][z] + P.beta * old[z];
-        } else {
-#pragma unroll
-          for (int z = 0; z < 8; ++z) acc[q][z] *= P.alpha;
-        }
-        if (whole) {
+            for (int z = 0; z < 8; ++z) acc[q][z] = fmaf(P.beta, old[z], acc[q][z]);
+          }
           __stcs(reinterpret_cast<uint4 *>(to), pack<VT>(acc[q]));
-        } else {
+        } else if (p < count) {
+          const int lo = p == 0 ? shift : 0, hi = min(8, k + shift - p * 8);
 #pragma unroll
           for (int z = 0; z < 8; ++z)
-            if (z >= lo && z < hi) to[z] = from_f32<VT>(acc[q][z]);
+            if (z >= lo && z < hi) {
+              float o = acc[q][z];
+              if (P.beta != 0.0f) o = fmaf(P.beta, to_f32(to[z]), o);
+              to[z] = from_f32<VT>(o);
+            }
         }
       }
     }
-    next.check(flag && r + step < P.m);
+    next.check(flag && r + step < P.m, P.err);
     s = next.s, e = next.e;
     entries(s, e);
     next.fetch(r + 2 * step);
@@ -227,45 +218,48 @@ sddmm_kernel(const WideParams<VT, IT> P, int wpr_log2) {
   const int64_t step = (int64_t)gridDim.x * ((NT / 32) >> wpr_log2);
   const int64_t r0 = (int64_t)blockIdx.x * ((NT / 32) >> wpr_log2) + (warp >> wpr_log2);
   const bool flag = lane == 0 && mine == 0;
+  const int k = (int)P.k;
   RowWalk<VT, IT> next(P);
   next.fetch(r0);
-  next.check(flag && r0 < P.m);
-  int64_t s = next.s, e = next.e;
+  next.check(flag && r0 < P.m, P.err);
+  IT s = next.s, e = next.e;
+  const uint32_t n = (uint32_t)min(P.n, (int64_t)0xffffffff);
   uint32_t first = s + mine < e ? (uint32_t)P.col[s + mine] : 0;
   next.fetch(r0 + step);
   for (int64_t r = r0; r < P.m; r += step) {
-    const DenseRow<VT> Y(P.Y + r * P.ldy, P.k);
-    const int shift = ALIGNED ? 0 : Y.shift;
-    for (int64_t i = s + mine; i < e; i += wpr) {
+    const DenseRow<VT> Y(P.Y + r * P.ldy, k);
+    const int shift = ALIGNED ? 0 : Y.shift, count = Y.count;
+    const int first_whole = shift > 0, last_whole = count - 1 - ((k + shift) % 8 != 0);
+    for (IT i = s + mine; i < e; i += wpr) {
       const uint32_t col = i == s + mine ? first : (uint32_t)P.col[i];
-      if (col >= (uint64_t)P.n) {
+      if (col >= n) {
         if (lane == 0) atomicOr(P.err, PF_DEVERR_BOUNDS);
         continue;
       }
-      const DenseRow<VT> X(P.X + (int64_t)col * P.ldx, P.k);
+      const DenseRow<VT> X(P.X + (int64_t)col * P.ldx, k);
+      const int delta = ALIGNED ? 0 : X.shift - shift;
       float acc[8] = {};
-      for (int v = lane; v < Y.count; v += 32 * Q) {
+      for (int v = lane; v < count; v += 32 * Q) {
         Gather<VT, ALIGNED> x[Q];
         uint4 y[Q];
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-          if (v + 32 * q < Y.count) {
-            x[q].load(X, v + 32 * q, shift);
+          if (v + 32 * q < count) {
+            x[q].load(X, v + 32 * q, delta);
             y[q] = __ldg(Y.piece + v + 32 * q);
           }
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
           const int p = v + 32 * q;
-          if (p >= Y.count) continue;
+          if (p >= count) continue;
           float f[8], g[8];
-          x[q].get(X.shift - shift, f);
+          x[q].get(delta, f);
           unpack<VT>(y[q], g);
-          const int lo = p == 0 ? shift : 0;
-          const int hi = (int)min((int64_t)8, P.k + shift - (int64_t)p * 8);
-          if (lo == 0 && hi == 8) {
+          if (p >= first_whole && p <= last_whole) {
 #pragma unroll
             for (int z = 0; z < 8; ++z) acc[z] = fmaf(f[z], g[z], acc[z]);
           } else {
+            const int lo = p == 0 ? shift : 0, hi = min(8, k + shift - p * 8);
 #pragma unroll
             for (int z = 0; z < 8; ++z)
               if (z >= lo && z < hi) acc[z] = fmaf(f[z], g[z], acc[z]);
@@ -280,7 +274,7 @@ sddmm_kernel(const WideParams<VT, IT> P, int wpr_log2) {
         P.dval[i] = from_f32<VT>(out);
       }
     }
-    next.check(flag && r + step < P.m);
+    next.check(flag && r + step < P.m, P.err);
     s = next.s, e = next.e;
     first = s + mine < e ? (uint32_t)P.col[s + mine] : 0;
     next.fetch(r + 2 * step);

@@ -50,7 +50,7 @@ static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, c
   // several pieces of columns at a time instead of several non-zeros
   const bool aligned = rows16(X, ldx) && rows16(Y, ldy);
   const bool few = nnz <= 2 * m;
-  const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? 4 : 1);
+  const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? (aligned ? 4 : 2) : 1);
   // threads a row: one for every unit of its columns, up to a CTA; the columns of
   // few rows are spread over more CTAs
   int tpr_log2 = 0;
@@ -61,8 +61,8 @@ static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, c
   if (ctas < h->num_sms) grid.y = (unsigned)std::min<int64_t>(64, ceil_div(units, 1 << tpr_log2));
   if (aligned && few) spmm_wide_kernel<VT, IT, 256, true, 1, 4><<<grid, 256, 0, st>>>(p, tpr_log2);
   else if (aligned) spmm_wide_kernel<VT, IT, 256, true, 4, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
-  else if (few) spmm_wide_kernel<VT, IT, 256, false, 1, 4><<<grid, 256, 0, st>>>(p, tpr_log2);
-  else spmm_wide_kernel<VT, IT, 256, false, 4, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else if (few) spmm_wide_kernel<VT, IT, 256, false, 1, 2><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else spmm_wide_kernel<VT, IT, 256, false, 2, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
   count_launches(1);
   PF_CUDA_TRY(cudaGetLastError());
   return PF_OK;
