@@ -51,10 +51,11 @@ static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, c
   const bool aligned = rows16(X, ldx) && rows16(Y, ldy);
   const bool few = nnz <= 2 * m;
   const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? (aligned ? 4 : 2) : 1);
-  // threads a row: one for every unit of its columns, up to a CTA; the columns of
-  // few rows are spread over more CTAs
+  // threads a row: one for every unit of its columns, up to a CTA, the power of
+  // two below (the one above leaves up to half of them idle); the columns of few
+  // rows are spread over more CTAs
   int tpr_log2 = 0;
-  while (tpr_log2 < 8 && (1 << tpr_log2) < units) ++tpr_log2;
+  while (tpr_log2 < 8 && (2 << tpr_log2) <= units) ++tpr_log2;
   while (tpr_log2 > 5 && ceil_div(m, 256 >> tpr_log2) < h->num_sms) --tpr_log2;
   const int64_t ctas = ceil_div(m, 256 >> tpr_log2), most = (int64_t)h->num_sms * (aligned ? 4 : 3);
   dim3 grid((unsigned)std::min(ctas, most));
