@@ -268,7 +268,11 @@ pf_status pf_distill_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
  * error word and treated as empty. 16-bit values, fp32 sums, rounded once;
  * alpha and beta are rounded to fp32; with beta == 0 Y is not read. Y must not
  * overlap X or W. Deterministic. Asynchronous on `stream`. rows, n, k and
- * groups are at most 2^31 - 1.                                              */
+ * groups are at most 2^31 - 1; stride_w may be 0 (one matrix for all groups).
+ * Arrays whose rows start on 16-byte boundaries run on the tensor cores, others
+ * on the CUDA cores. A call with few tiles cuts its sums into parts, whose
+ * scratch the handle keeps: the first call of its size allocates (make it
+ * before a stream capture).                                                 */
 pf_status pf_gmm_f16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
                          const int32_t *group_ptr, const uint16_t *X, int64_t ldx,
                          const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,

@@ -46,6 +46,10 @@ struct GmmTcParams {
   OT *C;
   int64_t ldc, stride_c;
   float alpha, beta;
+  int parts;               // SPLIT: parts of each sum, at least 2
+  int64_t most;            // SPLIT: tiles that there is scratch for
+  float *partial;          // SPLIT: 128 * BN floats for each tile and part
+  unsigned *arrived;       // SPLIT: 4 counters for each tile, 0 between calls
   bool aligned;            // C's rows start on 16-byte boundaries
   bool plain;              // 16-bit C, aligned, beta = 0
   unsigned *err;
@@ -186,6 +190,9 @@ struct GmmCfg {
   static constexpr int SMEM = STAGES * STAGE + 4 * GMM_STAGING + 1024;  // and alignment
 };
 
+// SPLIT: a tile's sum is cut into parts where there are too few tiles to fill the
+// GPU (a decoding step, a narrow layer): see the epilogue. 17 rows, n 512, k
+// 2048, one group: 4 tiles of 32 blocks each become 32 parts.
 constexpr uint64_t GMM_WAIT_NS = 4000000000ull;
 
 // columns that the matrix instruction computes for jn outputs
@@ -200,18 +207,20 @@ struct GmmTile {
   int i0;          // first i of the CTA (pair)
   int64_t j0;      // first j: an absolute row (FWD, DX) or a column of dY (DW)
   int jn;          // number of j
-  int64_t p0;      // DW: first row of the group
+  int64_t p0;      // first of p (DW: a row)
   int np;          // length of the sum
+  int64_t tile;    // SPLIT: the tile's number
+  int part;        // SPLIT: which part of its sum
 };
 
-template <int MODE, int CG, int BN, typename IT, typename OT>
+template <int MODE, int CG, int BN, bool SPLIT, typename IT, typename OT>
 struct GmmTiles {
   using Cfg = GmmCfg<MODE, CG, BN>;
   const GmmTcParams<IT, OT> &P;
   GroupWalk<IT> walk;
   int ti, tj;
-  int64_t t, step;
-  int64_t g = 0;           // DW: the next tile's group and place in it
+  int64_t t, step;         // items: tiles, or (SPLIT) parts of tiles
+  int64_t g = 0;           // DW: the next item's group and place in it
   int l = 0, step_l = 0;
   int64_t step_g = 0;
 
@@ -219,7 +228,7 @@ struct GmmTiles {
       : P(p), walk{p.ptr, p.groups, p.rows, p.err}, ti((p.ni + Cfg::TI - 1) / Cfg::TI),
         tj(MODE == GMM_DW ? (p.nj + BN - 1) / BN : 0), t(blockIdx.x / CG), step(gridDim.x / CG) {
     if constexpr (MODE == GMM_DW) {
-      const int64_t per = (int64_t)ti * tj;
+      const int64_t per = (int64_t)ti * tj * (SPLIT ? P.parts : 1);
       g = t / per;
       l = (int)(t - g * per);
       step_g = step / per;
@@ -231,16 +240,21 @@ struct GmmTiles {
   __device__ __forceinline__ bool next(GmmTile *o) {
     if constexpr (MODE == GMM_DW) {
       if (g >= P.groups) return false;
+      const int parts = SPLIT ? P.parts : 1;
+      const int l = this->l / parts;
+      if (SPLIT) o->tile = t / parts, o->part = this->l - l * parts;
       o->g = g;
       o->np = (int)group_rows(P.ptr, o->g, P.rows, &o->p0, P.err);
       o->i0 = l % ti * Cfg::TI;
       o->j0 = (int64_t)(l / ti) * BN;
       o->jn = min(BN, P.nj - (int)o->j0);
       g += step_g;
-      l += step_l;
-      if (l >= ti * tj) l -= ti * tj, ++g;
+      this->l += step_l;
+      if (this->l >= ti * tj * parts) this->l -= ti * tj * parts, ++g;
     } else {
+      const int64_t t = SPLIT ? this->t / P.parts : this->t;
       if (!walk.seek(t, BN, ti)) return false;
+      if (SPLIT) o->tile = t, o->part = (int)(this->t - t * P.parts);
       // rows and n fit 31 bits, and so do a group's row tiles; its tiles may not
       const int64_t l = t - walk.before;
       const int jt = l <= INT32_MAX ? (int)l / ti : (int)(l / ti);
@@ -255,12 +269,23 @@ struct GmmTiles {
       o->np = P.np;
       o->p0 = 0;
     }
-    t += step;
+    this->t += step;
+    if (SPLIT && o->tile >= P.most) {  // groups that overlap: no valid pointers
+      atomicOr(P.err, PF_DEVERR_ROWPTR);
+      return false;
+    }
+    if (SPLIT) {  // whole blocks of 64; a part of a short sum can be empty
+      const int64_t nb = (o->np + 63) / 64;
+      const int b0 = (int)(nb * o->part / P.parts), b1 = (int)(nb * (o->part + 1) / P.parts);
+      o->np = min(o->np, b1 * 64) - b0 * 64;
+      if (o->np < 0) o->np = 0;
+      o->p0 += b0 * 64;
+    }
     return true;
   }
 };
 
-template <int MODE, int CG, int BN, bool BF16, typename IT, typename OT>
+template <int MODE, int CG, int BN, bool BF16, bool SPLIT, typename IT, typename OT>
 __global__ void __launch_bounds__(GmmCfg<MODE, CG, BN>::NT, 1)
 gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   using Cfg = GmmCfg<MODE, CG, BN>;
@@ -303,7 +328,7 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
     return false;
   };
 
-  GmmTiles<MODE, CG, BN, IT, OT> tiles(P);
+  GmmTiles<MODE, CG, BN, SPLIT, IT, OT> tiles(P);
   GmmTile t;
   if (wid == 0) {  // ---- copies
     const uint32_t full_at = CG == 2 ? tc::map_rank(tc::smem_addr(&full[0]), 0)
@@ -315,6 +340,7 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       const int ncols = instr_cols<CG>(t.jn), half = ncols / CG;
       const int gw = (int)t.g * P.group_step;
       const int ia = t.i0 + (int)rank * 128;
+      const int p_first = SPLIT ? (int)t.p0 : 0;  // (DW reads t.p0)
       for (int kb = 0; kb < nb; ++kb, ++it) {
         const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
         if (!wait(&empty[s], ph ^ 1)) {
@@ -347,15 +373,16 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
                   &full[s], (uint32_t)(CG * (Cfg::A_BYTES + boxes * Cfg::BOX * 128)));
               if (CG == 2) ptx::mbar_arrive(&full[s]);
             }
+            const int p = p_first + kb * 64;
             if constexpr (MODE == GMM_FWD) {
-              tc::load_3d<CG>(sa, &M.a, bar, kb * 64, ia, gw);
+              tc::load_3d<CG>(sa, &M.a, bar, p, ia, gw);
             } else {
-              tc::load_3d<CG>(sa, &M.a, bar, ia, kb * 64, gw);
-              tc::load_3d<CG>(sa + 8192, &M.a, bar, ia + 64, kb * 64, gw);
+              tc::load_3d<CG>(sa, &M.a, bar, ia, p, gw);
+              tc::load_3d<CG>(sa + 8192, &M.a, bar, ia + 64, p, gw);
             }
             const int row = (int)t.j0 + (int)rank * half;
             for (int x = 0; x < boxes; ++x)
-              tc::load_2d<CG>(sb + x * Cfg::BOX * 128, &M.b, bar, kb * 64, row + x * Cfg::BOX);
+              tc::load_2d<CG>(sb + x * Cfg::BOX * 128, &M.b, bar, p, row + x * Cfg::BOX);
           }
         }
         __syncwarp();
@@ -455,7 +482,52 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
         }
       };
       const int ni = min(32, P.ni - i0);
-      if (BN >= 64 && sizeof(OT) == 2 && sum && P.plain) {
+      if constexpr (SPLIT) {
+        // this warp's 32 of i: the part's sum goes to memory, and the warp that
+        // brings the last part adds all of them, in their order
+        const int64_t mine = (int64_t)quad * 32 * BN + lane, item = 128 * BN;
+        float *to = P.partial + (t.tile * P.parts + t.part) * item + mine;
+        for (int j = 0; j < t.jn; j += 32) {
+          float v[32] = {};
+          if (sum) tc::tmem_load32(src + j, v);
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (j + x < t.jn) __stcg(to + (j + x) * 32, v[x]);
+        }
+        if (sum) release();
+        __threadfence();
+        __syncwarp();
+        unsigned before = 0;
+        unsigned *arrived = P.arrived + t.tile * 4 + quad;
+        if (lane == 0) before = atomicAdd(arrived, 1u);
+        if (__shfl_sync(~0u, before, 0) + 1 < (unsigned)P.parts) continue;
+        if (lane == 0) *arrived = 0;
+        __threadfence();
+        const float *from = P.partial + t.tile * P.parts * item + mine;
+        for (int j = 0; j < t.jn; j += 32, c += 32 * P.ldc) {
+          float v[32] = {};
+          for (int p = 0; p < P.parts; p += 4) {  // four parts on their way at once
+            float w[4][32];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int x = 0; x < 32; ++x)
+                w[y][x] = p + y < P.parts && j + x < t.jn
+                              ? __ldcg(from + (p + y) * item + (j + x) * 32)
+                              : 0.0f;
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int x = 0; x < 32; ++x) v[x] += w[y][x];
+          }
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            *reinterpret_cast<float *>(stage + x * 144 + lane * 4) = v[x];
+          __syncwarp();
+          store_floats(stage, c, P.ldc, ni, min(32, t.jn - j), P.alpha, P.beta, P.aligned);
+          __syncwarp();
+        }
+      } else if (BN >= 64 && sizeof(OT) == 2 && sum && P.plain) {
         for (int j = 0; j < t.jn; j += 64, c += 64 * P.ldc) {
           stage_pairs<OT>(stage, src + j, P.alpha);
           if (j + 64 >= t.jn) release();

@@ -347,3 +347,68 @@ def test_refusals(pf):
         assert pf.lib.pf_gmm_wgrad_bf16_i32(*a) == 1, at
     assert h.device_error() == 0
     h.close()
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("lengths,n,k", [([17], 512, 2048), ([3, 0, 300, 1], 264, 1000),
+                                         ([2100], 136, 72), ([1500, 0, 33, 1000], 128, 264)])
+def test_split_sums(pf, mode, lengths, n, k):
+    """Few tiles: their sums are cut into parts and joined, with alpha and beta,
+    uneven last parts, and rows before and after the groups."""
+    check(pf, lengths, n, k, mode, "bf16", 0.5, -1.0, start=2, after=3, seed=11)
+    check(pf, lengths, n, k, mode, "f16", out="f32" if mode == "dw" else "same", seed=12)
+
+
+def test_split_sums_leave_no_trace(pf):
+    """The joins' counters are back at zero after every call: calls of other
+    shapes through the same handle, in any order, give the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    h = pf.Handle()
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    cases = [(pointers([17]), r(17, 2048), r(1, 512, 2048)),
+             (pointers([5, 90, 0, 1]), r(96, 512), r(4, 256, 512)),
+             (pointers([400]), r(400, 1024), r(1, 128, 1024))]
+    outs = []
+    for _ in range(3):
+        for ptr, X, W in cases:
+            Y = torch.empty(X.shape[0], W.shape[1], dtype=X.dtype, device="cuda")
+            dW = torch.empty_like(W)
+            pf.grouped_mm(h, ptr, X, W, Y)
+            pf.grouped_wgrad(h, ptr, Y, X, dW)
+            outs.append((Y, dW))
+    for i, (Y, dW) in enumerate(outs):
+        assert torch.equal(Y, outs[i % 3][0]) and torch.equal(dW, outs[i % 3][1])
+    assert h.device_error() == 0
+    h.close()
+
+
+def test_overlapping_groups_are_flagged(pf):
+    """Pointers that go back and forth name more rows than there are: flagged,
+    and nothing is written outside of the scratch made for valid ones."""
+    h = pf.Handle()
+    dt = torch.bfloat16
+    ptr = torch.tensor([0, 20] * 40 + [0], dtype=torch.int32, device="cuda")
+    X, W = torch.ones(20, 512, dtype=dt, device="cuda"), torch.ones(80, 64, 512, dtype=dt, device="cuda")
+    Y = torch.zeros(20, 64, dtype=dt, device="cuda")
+    pf.grouped_mm(h, ptr, X, W, Y)
+    assert h.device_error() == 4
+    pf.grouped_mm(h, pointers([20] + [0] * 79), X, W, Y)
+    assert h.device_error() == 0 and bool((Y == 512).all())
+    h.close()
+
+
+def test_one_matrix_for_all_groups(pf):
+    """W expanded to all groups (distance 0 between matrices)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    X, W = (torch.randn(*s, generator=g, device="cuda").bfloat16() for s in ((90, 72), (1, 40, 72)))
+    ptr = pointers([30, 0, 60])
+    h = pf.Handle()
+    for w in (W, W[:, :, :71]):
+        k = w.shape[2]
+        Y, Z = torch.empty(90, 40, dtype=X.dtype, device="cuda"), torch.empty(90, 40, dtype=X.dtype, device="cuda")
+        pf.grouped_mm(h, ptr, X[:, :k], w.expand(3, 40, k), Y)
+        pf.grouped_mm(h, ptr, X[:, :k], w.repeat(3, 1, 1), Z)
+        # (another leading dimension may take the other kernel: another order of sums)
+        within(Y, Z.double(), 2 * UNIT["bf16"] * Z.double().abs() + 1e-4)
+    assert h.device_error() == 0
+    h.close()
