@@ -210,9 +210,9 @@ spmm_wide_kernel(const WideParams<VT, IT> P, int tpr_log2) {
 // dense rows on their way to a lane. The next row's bounds and first column are
 // fetched ahead, as above.
 template <typename VT, typename IT, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(NT, 4)
+__global__ void __launch_bounds__(NT, 3)
 sddmm_kernel(const WideParams<VT, IT> P, int wpr_log2) {
-  constexpr int Q = ALIGNED ? 4 : 2;
+  constexpr int Q = ALIGNED ? 4 : 3;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wpr = 1 << wpr_log2, mine = warp & (wpr - 1);
   const int64_t step = (int64_t)gridDim.x * ((NT / 32) >> wpr_log2);

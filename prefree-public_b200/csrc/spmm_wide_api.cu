@@ -50,19 +50,22 @@ static pf_status launch_spmm16(pf_handle h, int64_t m, int64_t n, int64_t nnz, c
   // several pieces of columns at a time instead of several non-zeros
   const bool aligned = rows16(X, ldx) && rows16(Y, ldy);
   const bool few = nnz <= 2 * m;
-  const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? (aligned ? 4 : 2) : 1);
+  const int64_t units = ceil_div(ceil_div((int64_t)k + (aligned ? 0 : 7), 8), few ? (aligned ? 4 : 3) : 1);
   // threads a row: one for every unit of its columns, up to a CTA, the power of
   // two below (the one above leaves up to half of them idle); the columns of few
   // rows are spread over more CTAs
   int tpr_log2 = 0;
-  while (tpr_log2 < 8 && (2 << tpr_log2) <= units) ++tpr_log2;
+  const int most_log2 = few ? 5 : 8;  // (what a row costs besides its pieces counts there)
+  while (tpr_log2 < 8 && (2 << tpr_log2) <= units &&
+         (tpr_log2 < most_log2 || ceil_div(m, 256 >> tpr_log2) < 4 * h->num_sms))
+    ++tpr_log2;
   while (tpr_log2 > 5 && ceil_div(m, 256 >> tpr_log2) < h->num_sms) --tpr_log2;
   const int64_t ctas = ceil_div(m, 256 >> tpr_log2), most = (int64_t)h->num_sms * (aligned ? 4 : 3);
   dim3 grid((unsigned)std::min(ctas, most));
   if (ctas < h->num_sms) grid.y = (unsigned)std::min<int64_t>(64, ceil_div(units, 1 << tpr_log2));
   if (aligned && few) spmm_wide_kernel<VT, IT, 256, true, 1, 4><<<grid, 256, 0, st>>>(p, tpr_log2);
   else if (aligned) spmm_wide_kernel<VT, IT, 256, true, 4, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
-  else if (few) spmm_wide_kernel<VT, IT, 256, false, 1, 2><<<grid, 256, 0, st>>>(p, tpr_log2);
+  else if (few) spmm_wide_kernel<VT, IT, 256, false, 1, 3><<<grid, 256, 0, st>>>(p, tpr_log2);
   else spmm_wide_kernel<VT, IT, 256, false, 2, 1><<<grid, 256, 0, st>>>(p, tpr_log2);
   count_launches(1);
   PF_CUDA_TRY(cudaGetLastError());
@@ -85,7 +88,7 @@ static pf_status launch_sddmm(pf_handle h, int64_t m, int64_t n, int64_t nnz, co
   int wpr_log2 = 0;
   while (wpr_log2 < 3 && ((int64_t)m << wpr_log2) < nnz) ++wpr_log2;
   const unsigned grid =
-      (unsigned)std::min<int64_t>(ceil_div(m, 8 >> wpr_log2), (int64_t)h->num_sms * 4);
+      (unsigned)std::min<int64_t>(ceil_div(m, 8 >> wpr_log2), (int64_t)h->num_sms * 3);
   if (rows16(X, ldx) && rows16(dY, lddy))
     sddmm_kernel<VT, IT, 256, true><<<grid, 256, 0, st>>>(p, wpr_log2);
   else sddmm_kernel<VT, IT, 256, false><<<grid, 256, 0, st>>>(p, wpr_log2);
