@@ -21,9 +21,10 @@
 // DW: rows past a group's end belong to the next group and must not meet the
 // sum (0 * NaN is NaN). A group's last, partial block is announced to a warp of
 // its own, which clears the rows up to the next multiple of 16 (what the matrix
-// instruction reads) in both operands before it passes the stage on. (Copying
-// the tail in boxes of 8 rows and single rows instead, filled up by boxes
-// outside of the array, cost 3 us a tile.)
+// instruction reads) in both operands before it passes the stage on. That takes
+// about as long as the ring looks ahead, so the block is loaded first and used
+// two blocks later. (Copied in boxes of 8 rows and single rows, filled up by
+// boxes outside of the array, it cost 3 us a tile.)
 #pragma once
 
 #include "gmm_common.cuh"
@@ -291,7 +292,7 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   using Cfg = GmmCfg<MODE, CG, BN>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[Cfg::STAGES], empty[Cfg::STAGES], acc_full[2], acc_empty[2];
-  __shared__ uint64_t tail[Cfg::STAGES];  // DW
+  __shared__ uint64_t tail[Cfg::STAGES], cleared[Cfg::STAGES];  // DW
   __shared__ uint32_t tmem_base;
   __shared__ volatile int dead;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -304,6 +305,7 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       ptx::mbar_init(&full[s], CG);
       ptx::mbar_init(&empty[s], 1);
       ptx::mbar_init(&tail[s], 1);
+      ptx::mbar_init(&cleared[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&acc_full[s], 1);
@@ -353,7 +355,9 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
           if constexpr (MODE == GMM_DW) {
             const int panels_b = (half + 63) / 64;
             const uint32_t bytes = (uint32_t)(2 + panels_b) * 8192;
-            const bool whole = t.np - kb * 64 >= 64;
+            // the partial block goes first
+            const bool ragged = (t.np & 63) != 0, whole = !ragged || kb > 0;
+            const int block = ragged ? (kb > 0 ? kb - 1 : nb - 1) : kb;
             const uint32_t to = whole ? bar : tc::smem_addr(&tail[s]);
             if (!whole) {
               ptx::mbar_arrive_expect_tx(&tail[s], bytes);
@@ -361,7 +365,7 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
               ptx::mbar_arrive_expect_tx(&full[s], CG * bytes);
               if (CG == 2) ptx::mbar_arrive(&full[s]);
             }
-            const int row = (int)t.p0 + kb * 64, jb = (int)t.j0 + (int)rank * half;
+            const int row = (int)t.p0 + block * 64, jb = (int)t.j0 + (int)rank * half;
             tc::load_2d<CG>(sa, &M.a, to, ia, row);
             tc::load_2d<CG>(sa + 8192, &M.a, to, ia + 64, row);
             for (int x = 0; x < panels_b; ++x)
@@ -404,42 +408,49 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       ok = wait(&acc_empty[buf], aph ^ 1);
       tc::fence_after_sync();
       const uint32_t d = tmem + buf * BN;
-      for (int kb = 0; ok && kb < nb; ++kb, ++it) {
-        const uint32_t s = it % Cfg::STAGES, ph = it / Cfg::STAGES & 1;
+      // DW: a partial block is loaded first and used after the next `late` ones, by
+      // when its rows are cleared
+      const bool ragged = MODE == GMM_DW && (t.np & 63) != 0;
+      const int late = min(nb - 1, 2);
+      for (int c = 0; ok && c < nb; ++c) {
+        const int kb = !ragged || c > late ? c : c < late ? c + 1 : 0;  // as loaded
+        const uint32_t n = it + kb, s = n % Cfg::STAGES, ph = n / Cfg::STAGES & 1;
         if (!wait(&full[s], ph)) {
           ok = false;
           break;
         }
-        // the other CTA's cleared rows (a wait of this scope at every block costs
-        // as much as two blocks)
-        if (CG == 2 && MODE == GMM_DW && t.np - kb * 64 < 64) tc::acquire_cluster(&full[s], ph);
         tc::fence_after_sync();
         if (tc::elect()) {
           const uint32_t sa = stage0 + s * Cfg::STAGE, sb = sa + Cfg::A_BYTES;
           const uint64_t da = tc::operand_desc(sa, 8192), db = tc::operand_desc(sb, 8192);
-          const int left = t.np - kb * 64;
+          const int left = ragged ? (kb > 0 ? 64 : t.np & 63) : t.np - kb * 64;
           // 16 along p: 32 bytes of a line, or two atoms of eight lines
           constexpr int STEP_A = MODE == GMM_FWD ? 2 : 128, STEP_B = MODE == GMM_DW ? 128 : 2;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (q * 16 < left)
-              tc::mma<CG>(d, da + q * STEP_A, db + q * STEP_B, idesc, kb + q > 0);
+              tc::mma<CG>(d, da + q * STEP_A, db + q * STEP_B, idesc, c + q > 0);
           tc::commit<CG>(&empty[s]);
-          if (kb + 1 == nb) tc::commit<CG>(&acc_full[buf]);
+          if (c + 1 == nb) tc::commit<CG>(&acc_full[buf]);
         }
         __syncwarp();
       }
+      it += nb;
     }
   } else if (MODE == GMM_DW && wid == 6) {  // ---- rows past a group's end
-    const uint32_t full_at = CG == 2 ? tc::map_rank(tc::smem_addr(&full[0]), 0)
-                                     : tc::smem_addr(&full[0]);
+    // The second CTA of a pair tells the first one's warp, which acquires its
+    // writes before it passes the stage on for both: the warp that issues the
+    // matrix instructions waits at its own CTA's scope alone (a wait at the
+    // cluster's costs it as much as two blocks).
+    const uint32_t leader = CG == 2 ? tc::map_rank(tc::smem_addr(&cleared[0]), 0) : 0;
     uint32_t it = 0, parity = 0;  // parity: one bit to a stage, flipped at each use
     while (tiles.next(&t)) {
       const int nb = (t.np + 63) / 64, valid = t.np & 63;
+      const uint32_t s = it % Cfg::STAGES;
       it += nb;
       if (valid == 0) continue;
-      const uint32_t s = (it - 1) % Cfg::STAGES;
-      if (!wait(&tail[s], parity >> s & 1)) break;
+      const uint32_t turn = parity >> s & 1;
+      if (!wait(&tail[s], turn)) break;
       parity ^= 1u << s;
       const int panels = 2 + (instr_cols<CG>(t.jn) / CG + 63) / 64;
       const int zero = ((valid + 15) & ~15) - valid;  // the matrix instruction reads no more
@@ -451,7 +462,17 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
       }
       ptx::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive_release(full_at + s * 8);
+      if (CG == 2 && rank != 0) {
+        if (lane == 0) tc::mbar_arrive_release(leader + s * 8);
+      } else {
+        if (CG == 2) {
+          if (!wait(&cleared[s], turn)) break;
+          tc::acquire_cluster(&cleared[s], turn);
+          __syncwarp();
+        }
+        if (lane == 0)
+          for (int x = 0; x < CG; ++x) ptx::mbar_arrive(&full[s]);
+      }
       __syncwarp();
     }
   } else if (wid >= 2) {  // ---- accumulator to C
