@@ -79,7 +79,7 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   PF_CHECK_ARG(sizeof(IT) == 8 || nnz <= INT32_MAX, "int32 row_ptr cannot index nnz=%lld",
                (long long)nnz);
   PF_CHECK_ARG(ldz >= n && (!dZ || lddz >= n), "leading dimension below n");
-  PF_CHECK_ARG((const void *)dZ != (const void *)Z || lddz == ldz,
+  PF_CHECK_ARG(!dZ || (const void *)dZ != (const void *)Z || lddz == ldz,
                "dZ in Z's place needs lddz == ldz");
   PF_CHECK_ARG(((uintptr_t)row_ptr % sizeof(IT)) == 0 && ((uintptr_t)col % 4) == 0 &&
                    ((uintptr_t)val % sizeof(VT)) == 0 && ((uintptr_t)Z % sizeof(VT)) == 0 &&
@@ -103,6 +103,7 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   p.dZ = dZ;
   p.lddz = lddz;
   p.inv_tau = (float)(1.0 / temperature);
+  if (n == 0) p.Z = nullptr, p.ldz = p.lddz = 0;  // no row has a piece to copy
   p.err = h->err;
   return dZ ? launch_rows<VT, IT, true>(h, p, st) : launch_rows<VT, IT, false>(h, p, st);
 }

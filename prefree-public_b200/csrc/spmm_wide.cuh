@@ -44,7 +44,7 @@ struct DenseRow {
   __device__ __forceinline__ DenseRow(const VT *row, int64_t k) {
     shift = (int)(((uintptr_t)row & 15) / sizeof(VT));
     piece = reinterpret_cast<const uint4 *>(row - shift);
-    count = (int)((k + shift + 7) / 8);
+    count = k > 0 ? (int)((k + shift + 7) / 8) : 0;
   }
 };
 

@@ -16,8 +16,8 @@ static pf_status check_wide(pf_handle h, int64_t m, int64_t n, int64_t nnz, cons
                (long long)nnz);
   PF_CHECK_ARG(n <= (int64_t)INT32_MAX + 1, "n must fit int32 column indices");
   PF_CHECK_ARG(nnz == 0 || n > 0, "nnz > 0 needs n > 0 (column indices lie in [0, n))");
-  PF_CHECK_ARG(row_ptr && Y, "null row_ptr or Y");
-  PF_CHECK_ARG(nnz == 0 || (col && val && X), "null col/val/X with nnz > 0");
+  PF_CHECK_ARG(row_ptr && (Y || k == 0), "null row_ptr or Y");
+  PF_CHECK_ARG(nnz == 0 || (col && val && (X || k == 0)), "null col/val/X with nnz > 0");
   PF_CHECK_ARG(ldy >= k && (nnz == 0 || ldx >= k), "leading dimension below k");
   PF_CHECK_ARG(((uintptr_t)row_ptr % sizeof(IT)) == 0 && ((uintptr_t)Y % sizeof(VT)) == 0 &&
                    (nnz == 0 || (((uintptr_t)col % 4) == 0 && ((uintptr_t)val % sizeof(VT)) == 0 &&

@@ -159,6 +159,49 @@ def test_no_rows_and_no_entries(pf):
     assert h.device_error() == 0
 
 
+def test_no_columns(pf):
+    """A vocabulary of nothing: losses of 0, and no read through any pointer."""
+    h = pf.Handle()
+    loss = torch.full((3,), math.nan, device="cuda")
+    ptr, some = pointers([0, 0, 0]), torch.zeros(8, device="cuda")
+    f = pf.lib.pf_distill_f32_i32
+    for z in (None, some.data_ptr() + 4):
+        assert f(h.ptr, 3, 0, 0, ptr.data_ptr(), None, None, 1.0, z, 5, None, loss.data_ptr(), None,
+                 0, None) == 0
+        torch.cuda.synchronize()
+        assert loss.tolist() == [0.0, 0.0, 0.0]
+        loss.fill_(math.nan)
+    assert h.device_error() == 0
+    h.close()
+
+
+@pytest.mark.parametrize("keep", [64, 65, 200])
+@pytest.mark.parametrize("n", [700, 20000])
+def test_kept_around_the_listed_number(pf, keep, n):
+    """Rows of up to 64 entries are listed by one warp, longer ones are not;
+    repeated columns in both, beside rows of weight 0 and rows without entries."""
+    lengths = [keep, 0, keep, 3, keep]
+    col, val, z = inputs(5, n, lengths, keep, distinct=False)
+    col[1] = col[0]
+    col[keep - 1] = col[0]
+    col[keep + 40] = col[keep + 2]
+    w = torch.tensor([1.0, 1.0, 0.0, 2.0, -0.5])
+    check(pf, lengths, col, val, z, "f32", w)
+    check(pf, lengths, col, val, z, "bf16", w, in_place=True)
+
+
+@pytest.mark.parametrize("rows", [300, 2500])
+def test_more_rows_than_clusters(pf, rows):
+    """Every cluster takes several rows, some of weight 0, some empty."""
+    g = torch.Generator().manual_seed(rows)
+    lengths = torch.randint(0, 70, (rows,), generator=g).tolist()
+    col, val, z = inputs(rows, 1025, lengths, rows)
+    w = torch.rand(rows, generator=g)
+    w[::7] = 0.0
+    check(pf, lengths, col, val, z, "f16", w, 1.1)
+    check(pf, lengths, col, val, z, "f16", w, 1.1, want=("loss",))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("n", [64, 9000])
 def test_infinities_and_masks(pf, dtype, n):

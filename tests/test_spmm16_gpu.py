@@ -186,6 +186,25 @@ def test_gradients_against_differences(pf):
     h.close()
 
 
+def test_no_columns(pf):
+    """Rows of length 0: nothing to write for the product, dval = beta * dval."""
+    h = pf.Handle()
+    dt, dev = torch.bfloat16, "cuda"
+    X, Y = torch.ones(5, 0, dtype=dt, device=dev), torch.zeros(3, 0, dtype=dt, device=dev)
+    ptr, col = pointers([2, 0, 1]), torch.zeros(3, dtype=torch.int32, device=dev)
+    d = torch.full((3,), 2.0, dtype=dt, device=dev)
+    pf.spmm(h, 3, 5, 3, ptr, col, d, X, Y)
+    pf.sddmm(h, 3, 5, 3, ptr, col, Y, X, d, beta=1.5)
+    assert d.tolist() == [3.0, 3.0, 3.0] and h.device_error() == 0
+    # the same through pointers that are not null: they are not read
+    some = torch.zeros(64, dtype=dt, device=dev)
+    p = some.data_ptr() + 2
+    assert pf.lib.pf_sddmm_bf16_i32(h.ptr, 3, 5, 3, ptr.data_ptr(), col.data_ptr(), 0, 1.0, p, 0, p,
+                                    0, 2.0, d.data_ptr(), None) == 0
+    assert d.tolist() == [6.0, 6.0, 6.0] and h.device_error() == 0
+    h.close()
+
+
 def test_bad_columns_and_pointers_are_flagged(pf):
     h = pf.Handle()
     dt, dev = torch.bfloat16, "cuda"
