@@ -5,6 +5,10 @@
  * int32 column indices, int32 or int64 row pointers. No preprocessing pass:
  * every call works straight from (row_ptr, col_idx, val) as given.
  *
+ * Further operators on the same CSR arrays: SpMM and the gradient of its
+ * values, distillation from a teacher's kept logits, matrix products grouped
+ * by rows.
+ *
  * Drop-in map onto wang-luhan/preFree-public:
  *   - the C++ entry point `preFreeSpMV` itself (include/PreFree.h:3-5,
  *     defined at src/spmv_kernel/preFreeSpMV.cu:563-662) is declared, with the

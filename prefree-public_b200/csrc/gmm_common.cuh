@@ -6,8 +6,7 @@
 // on the device (the group sizes are never read back to the host).
 #pragma once
 
-#include "distill.cuh"
-#include "pf_common.cuh"
+#include "pf_values.cuh"
 
 namespace pf {
 

@@ -18,6 +18,15 @@
 // Tiles are found on the device from group_ptr (GroupWalk), by each role for
 // itself.
 //
+// Measured: 16384 rows, one group, n 4096, k 2048, bf16: 160-166 us alone
+// (1660-1720 TFLOP/s; cuBLAS's product of the same size 164-171), 207 us in a
+// long run under the power cap (cuBLAS 201-208); 16 groups of 1024 rows 170-178
+// and 230 us; 64 groups of 128 rows, 2048 x 2048: 102-113 us, 82 us of it the
+// weights' bytes. Large products are bound by the tensor cores and the power
+// cap, products of few rows by the weights' bytes, gradients of few rows by
+// their own: 64 of 2048 x 2048 over 64 rows each take 140 us, as does setting
+// those bytes to zero.
+//
 // DW: rows past a group's end belong to the next group and must not meet the
 // sum (0 * NaN is NaN). A group's last, partial block is announced to a warp of
 // its own, which clears the rows up to the next multiple of 16 (what the matrix
@@ -61,8 +70,9 @@ struct GmmTcParams {
 // results as pairs of columns through transposing matrix stores (lines of 64
 // bytes), everything else as floats (lines of 128 bytes); 16 bytes of padding
 // to a line keep the banks apart. Storing straight from the registers, 2 bytes
-// a lane and 64 bytes an instruction, bound the kernel: 790 us against 82 us of
-// DRAM time for 64 gradients of 2048 x 2048.
+// a lane and 64 bytes an instruction, bound the kernel: 790 us instead of 140
+// for 64 gradients of 2048 x 2048. (Rows of 256 bytes put together by all four
+// warps take 140 too.)
 constexpr int GMM_STAGING = 64 * (64 + 16);  // and 32 * (128 + 16) is less
 
 template <typename OT>
@@ -101,7 +111,8 @@ __device__ __forceinline__ void stage_pairs(uint8_t *stage, uint32_t src, float 
                          pack2<OT>(alpha * hi[2], alpha * hi[3]));
   }
 }
-// C's rows are 16-byte aligned; ni of 32 i and nj of 64 j exist
+// ... to C (zeros where `stage` is null), whose rows are 16-byte aligned; ni of 32
+// i and nj of 64 j exist
 template <typename OT>
 __device__ __forceinline__ void store_pairs(const uint8_t *stage, OT *c, int64_t ldc, int ni,
                                             int nj) {
@@ -111,14 +122,15 @@ __device__ __forceinline__ void store_pairs(const uint8_t *stage, OT *c, int64_t
   if (ni == 32 && nj == 64) {
     uint4 v[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const uint4 *>(from + q * 640);
+    for (int q = 0; q < 8; ++q)
+      v[q] = stage ? *reinterpret_cast<const uint4 *>(from + q * 640) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4 *>(p + q * 8 * ldc) = v[q];
     return;
   }
 #pragma unroll 1
   for (int j = lane >> 2; j < nj; j += 8, from += 640, p += 8 * ldc) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+    const uint4 v = stage ? *reinterpret_cast<const uint4 *>(from) : make_uint4(0, 0, 0, 0);
     if (x * 8 + 8 <= ni) {
       *reinterpret_cast<uint4 *>(p) = v;
     } else {
@@ -181,12 +193,12 @@ template <int MODE, int CG, int BN>
 struct GmmCfg {
   static constexpr int TI = 128 * CG;           // i of a tile
   static constexpr int BH = BN / CG;            // B rows that one CTA loads
-  static constexpr int BOX = BH < 32 ? BH : 32; // rows of one B box (FWD, DX)
+  static constexpr int BOX = 32;                // rows of one B box (FWD, DX)
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BH * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 200 * 1024 / STAGE > 10 ? 10 : 200 * 1024 / STAGE;
-  static constexpr int COLS = 2 * BN < 32 ? 32 : 2 * BN;  // tensor memory columns
+  static constexpr int STAGES = 200 * 1024 / STAGE;
+  static constexpr int COLS = 2 * BN;           // tensor memory columns
   static constexpr int NT = MODE == GMM_DW ? 224 : 192;
   static constexpr int SMEM = STAGES * STAGE + 4 * GMM_STAGING + 1024;  // and alignment
 };
@@ -548,12 +560,12 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
           store_floats(stage, c, P.ldc, ni, min(32, t.jn - j), P.alpha, P.beta, P.aligned);
           __syncwarp();
         }
-      } else if (BN >= 64 && sizeof(OT) == 2 && sum && P.plain) {
+      } else if (sizeof(OT) == 2 && P.plain) {
         for (int j = 0; j < t.jn; j += 64, c += 64 * P.ldc) {
-          stage_pairs<OT>(stage, src + j, P.alpha);
-          if (j + 64 >= t.jn) release();
+          if (sum) stage_pairs<OT>(stage, src + j, P.alpha);
+          if (sum && j + 64 >= t.jn) release();
           else __syncwarp();
-          store_pairs(stage, c, P.ldc, ni, min(64, t.jn - j));
+          store_pairs(sum ? stage : nullptr, c, P.ldc, ni, min(64, t.jn - j));
           __syncwarp();
         }
       } else {
