@@ -187,8 +187,9 @@ __device__ __forceinline__ void subtract_many(const DistillParams<VT, IT> &P, co
 // entries' columns, written over what the others stored. Nothing in the common
 // case waits for it but the release of the slots, which also keeps it within
 // STAGES + 2 rows of the others: the DISTILL_RING rows kept apart are enough.
-// Rows of more than DISTILL_LIST entries are told to the others, who look through the entries for columns that they hold and
-// subtract p (subtract_many). Repeated columns add up in the entries' order.
+// Of rows of more than DISTILL_LIST entries the others wait to be told the
+// teacher's statistics; they look through the entries for columns that they hold
+// and subtract p (subtract_many). Repeated columns add up in the entries' order.
 template <typename VT, typename IT, int NT, bool GRAD>
 __global__ void __launch_bounds__(NT + 64, DistillCfg<VT, NT>::CTAS)
 distill_kernel(const DistillParams<VT, IT> P) {
@@ -341,8 +342,8 @@ distill_kernel(const DistillParams<VT, IT> P) {
         if (term.as != 0.0f && term.qs == 0.0f) v = (double)term.w * INFINITY;
         else if (term.as != 0.0f)
           v = (double)term.w *
-              (((double)term.d - (double)term.am + (double)term.qm) *
-                   (double)P.inv_tau + log((double)term.qs / (double)term.as));
+              (((double)term.d - (double)term.am + (double)term.qm) * (double)P.inv_tau +
+               log((double)term.qs / (double)term.as));
         P.loss[term.r] = (float)v;
       }
       term.r = -1;
@@ -454,7 +455,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
       }
       a.s = warp_sum(a.s);
       const float gt = w * P.inv_tau / a.s;  // not used without mass
-      if (GRAD && !listing) {
+      if (GRAD) {  // for every row: the barrier's phase counts them
         if (lane == 0) {
           told_as[ring] = make_float2(a.m, a.s == 0.0f ? 0.0f : gt);
           ptx::mbar_arrive(&told[ring]);
@@ -532,6 +533,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
           if (mine) last.repeats |= (atomicOr(&seen[c_[u] / 32 % 512], bit) & bit) != 0;
         }
         last.repeats = __any_sync(~0u, last.repeats);
+        __syncwarp();
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (last.c[u] != 0xffffffffu) seen[c_[u] / 32 % 512] = 0;

@@ -202,6 +202,30 @@ def test_more_rows_than_clusters(pf, rows):
     check(pf, lengths, col, val, z, "f16", w, 1.1, want=("loss",))
 
 
+@pytest.mark.parametrize("n,rows", [(150, 30000), (5000, 3000)])
+def test_long_rows_among_many_short_ones(pf, n, rows):
+    """Clusters take tens of rows each, of which now and then one has more
+    entries than are listed: the first such row of a cluster can be any of them.
+    The rows repeat a few, so that 64-bit results are computed for those alone."""
+    kinds = 53
+    lengths = [100 if r % 17 == 5 else r % 4 for r in range(kinds)]
+    col, val, z = inputs(kinds, n, lengths, n)
+    w = torch.ones(kinds)
+    w[7] = 0.0
+    z, val = z.bfloat16(), val.bfloat16()
+    rl, rd, pl, pd = formulas(lengths, col, val, z, w, 1.0)
+    start = [0]
+    for c in lengths:
+        start.append(start[-1] + c)
+    kind = torch.randint(0, kinds, (rows,), generator=torch.Generator().manual_seed(rows))
+    at = torch.cat([torch.arange(start[k], start[k + 1]) for k in kind.tolist()])
+    loss, dz, err = run(pf, [lengths[k] for k in kind.tolist()], col[at], val[at], z[kind], "bf16",
+                        w[kind])
+    assert err == 0
+    within(loss, rl[kind], (EPS * pl + 2.0 ** -23 * rl.abs() + 1e-37)[kind])
+    within(dz, rd[kind], (UNIT["bf16"] * rd.abs() + EPS * pd + TINY["bf16"])[kind])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("n", [64, 9000])
 def test_infinities_and_masks(pf, dtype, n):
