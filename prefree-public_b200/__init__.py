@@ -337,7 +337,7 @@ def _stream(stream, t) -> int:
 
 def _ld(t, what: str, rows: int, cols: int, dtype) -> int:
     """The leading dimension of a row-major rows x cols CUDA tensor."""
-    if t.shape != (rows, cols) or t.dtype != dtype or not t.is_cuda:
+    if t.shape != (rows, cols) or t.dtype is not dtype or not t.is_cuda:
         raise PfError(1, f"{what}: a CUDA tensor of {(rows, cols)} {dtype} is wanted, not of "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     ld, inner = t.stride()
@@ -349,8 +349,8 @@ def _ld(t, what: str, rows: int, cols: int, dtype) -> int:
 def _flat(t, what: str, least: int, dtype, exact: bool = False) -> int:
     """The address of a contiguous 1-d CUDA tensor of at least (or exactly)
     `least` elements."""
-    if not t.is_cuda or t.dtype != dtype or t.dim() != 1 or t.shape[0] < least or \
-            (exact and t.shape[0] != least) or not t.is_contiguous():
+    if not t.is_cuda or t.dtype is not dtype or t.dim() != 1 or t.numel() < least or \
+            (exact and t.numel() != least) or not t.is_contiguous():
         raise PfError(1, f"{what}: a contiguous 1-d CUDA tensor of {'' if exact else 'at least '}"
                          f"{least} {dtype} is wanted, not {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
