@@ -95,7 +95,8 @@ struct DistillCfg {
   static constexpr int PIECE = NT * NV;            // pieces of a slot
   static constexpr int NW = NT / 32;
   static constexpr int STAGES = 3;
-  static constexpr int CTAS = NT >= 256 ? 2 : 4;   // per SM
+  // per SM (64 threads: 6 instead of 4 took 15-20 % off vocabularies up to 4000)
+  static constexpr int CTAS = NT >= 256 ? 2 : NT >= 128 ? 4 : 6;
   static constexpr int SMEM = STAGES * PIECE * 16;
 };
 
