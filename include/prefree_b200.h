@@ -162,7 +162,7 @@ pf_status pf_spmm_f32_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
  * model's dispatch and combine: A holds the gates (tokens x slots, a few
  * non-zeros to a row), X the slots' rows. All k columns in one pass over A;
  * sums in fp32 in the row's order, rounded once; alpha and beta are rounded to
- * fp32. Deterministic. Y must not overlap X.                                */
+ * fp32. Deterministic. Y must not overlap X. k is at most 2^31 - 65.        */
 pf_status pf_spmm_f16_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
                           const int32_t *row_ptr, const int32_t *col_idx,
                           const uint16_t *val, int k, double alpha, const uint16_t *X,
@@ -272,7 +272,7 @@ pf_status pf_distill_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
  * error word and treated as empty. 16-bit values, fp32 sums, rounded once;
  * alpha and beta are rounded to fp32; with beta == 0 Y is not read. Y must not
  * overlap X or W. Deterministic. Asynchronous on `stream`. rows, n, k and
- * groups are at most 2^31 - 1; stride_w may be 0 (one matrix for all groups).
+ * groups are at most 2^31 - 1025; stride_w may be 0 (one matrix for all groups).
  * Arrays whose rows start on 16-byte boundaries run on the tensor cores, others
  * on the CUDA cores. A call with few tiles cuts its sums into parts, whose
  * scratch the handle keeps: the first call of its size allocates (make it

@@ -8,6 +8,9 @@
 
 namespace pf {
 
+// largest size: the kernels' 32-bit coordinates run up to a tile past the end
+constexpr int64_t kMost = INT32_MAX - 1024;
+
 // cuTensorMapEncodeTiled, looked up at run time (the library does not link
 // against the driver); null where there is none
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
@@ -193,8 +196,8 @@ static pf_status launch_gmm(pf_handle h, int64_t groups, int64_t rows, int64_t n
                "negative size (groups=%lld rows=%lld n=%lld k=%lld)", (long long)groups,
                (long long)rows, (long long)n, (long long)k);
   if (groups == 0 || rows == 0 || n == 0) return PF_OK;
-  PF_CHECK_ARG(groups < INT32_MAX && n <= INT32_MAX && k <= INT32_MAX && rows <= INT32_MAX,
-               "groups, rows, n and k must fit 31 bits");
+  PF_CHECK_ARG(groups <= kMost && n <= kMost && k <= kMost && rows <= kMost,
+               "groups, rows, n and k must be at most 2^31 - 1025");
   PF_CHECK_ARG(ptr && Y, "null group_ptr or Y");
   PF_CHECK_ARG(k == 0 || (X && W), "null X/W with k > 0");
   const int64_t wcols = trans_w ? k : n, wrows = trans_w ? n : k;
@@ -238,8 +241,8 @@ static pf_status launch_wgrad(pf_handle h, int64_t groups, int64_t rows, int64_t
                "negative size (groups=%lld rows=%lld n=%lld k=%lld)", (long long)groups,
                (long long)rows, (long long)n, (long long)k);
   if (groups == 0 || n == 0 || k == 0) return PF_OK;
-  PF_CHECK_ARG(groups < INT32_MAX && n <= INT32_MAX && k <= INT32_MAX && rows <= INT32_MAX,
-               "groups, rows, n and k must fit 31 bits");
+  PF_CHECK_ARG(groups <= kMost && n <= kMost && k <= kMost && rows <= kMost,
+               "groups, rows, n and k must be at most 2^31 - 1025");
   PF_CHECK_ARG(ptr && dW, "null group_ptr or dW");
   PF_CHECK_ARG(rows == 0 || (dY && X), "null dY/X with rows > 0");
   PF_CHECK_ARG((rows == 0 || (lddy >= n && ldx >= k)) && lddw >= k,

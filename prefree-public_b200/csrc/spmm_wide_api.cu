@@ -15,6 +15,7 @@ static pf_status check_wide(pf_handle h, int64_t m, int64_t n, int64_t nnz, cons
   PF_CHECK_ARG(sizeof(IT) == 8 || nnz <= INT32_MAX, "int32 row_ptr cannot index nnz=%lld",
                (long long)nnz);
   PF_CHECK_ARG(n <= (int64_t)INT32_MAX + 1, "n must fit int32 column indices");
+  PF_CHECK_ARG(k <= INT32_MAX - 64, "k must be at most 2^31 - 65");
   PF_CHECK_ARG(nnz == 0 || n > 0, "nnz > 0 needs n > 0 (column indices lie in [0, n))");
   PF_CHECK_ARG(row_ptr && (Y || k == 0), "null row_ptr or Y");
   PF_CHECK_ARG(nnz == 0 || (col && val && (X || k == 0)), "null col/val/X with nnz > 0");
