@@ -87,6 +87,11 @@ constexpr uint64_t DISTILL_WAIT_NS = 4000000000ull;
 constexpr int DISTILL_MAX_C = 8;    // CTAs of a cluster
 constexpr int DISTILL_LIST = 64;    // entries of a row that the teacher's warp lists
 constexpr int DISTILL_RING = 16;    // rows whose barriers and results are kept apart
+// 2^(scale (x - m)) is taken as 2^(scale x - ms), ms = scale m rounded, and one
+// more factor corrects that rounding, which a whole sum shares: a power within
+// 1/2 of 0 as long as |ms| is at most 2^24. (From 2^31 on the power leaves fp32's
+// range: inf * 0.) Above, the difference is taken first.
+constexpr float DISTILL_FOLDED = 16777216.0f;
 
 template <typename VT, int NT>
 struct DistillCfg {
@@ -636,9 +641,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
           for (int e = 0; e < VE; ++e) m = fmaxf(m, x[e]);
         });
         const float ms = m * scale;
-        if (fabsf(ms) <= 1e30f) {
-          // 2^(scale (x - m)) as 2^(scale x - ms); one more factor corrects the
-          // rounding of ms, which all of them share
+        if (fabsf(ms) <= DISTILL_FOLDED) {
           pieces(v0, [&](int j, int v, bool cut) {
             float x[VE];
             values(slot[j * NT], v, cut, x);
@@ -647,7 +650,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
           });
           sum[0] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * exp2_fast(-fmaf(m, scale, -ms));
         } else {
-          // the type's lowest values, or infinities: no product may overflow
+          // masks (finite ones of any size too) and infinities
           const float b = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
           for (int j = 0; j < NV; ++j) {
@@ -699,7 +702,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
           }
           const uint4 *slot = reinterpret_cast<const uint4 *>(slots) + (size_t)s * PIECE;
           const int v0 = (c * (int)C + (int)rank) * PIECE;
-          if (!many && fabsf(ms) <= 1e30f && same) {
+          if (!many && fabsf(ms) <= DISTILL_FOLDED && same) {
             uint4 *to = reinterpret_cast<uint4 *>(dz - shift);
             pieces(v0, [&](int j, int v, bool cut) {
               float x[VE];

@@ -254,6 +254,56 @@ def test_infinities_and_masks(pf, dtype, n):
     assert float(dz[4].abs().sum()) == 0.0
 
 
+@pytest.mark.parametrize("dtype,sizes", [
+    ("bf16", (1e6, 1e8, 3e9, 1e10, 1e12, 1e15, 1e20, 1e30)),
+    ("f32", (1e6, 1e8, 3e9, 1e10, 1e12, 1e15, 1e20, 1e30)), ("f16", (6e4,) * 8)])
+@pytest.mark.parametrize("tau", [0.1, 1.0, 2.0])
+@pytest.mark.parametrize("kind", ["half", "most", "high"])
+@pytest.mark.parametrize("n", [700, 40001, 300001])
+def test_finite_masks_of_any_size(pf, dtype, sizes, tau, kind, n):
+    """Finite logits far below all others, as masks are written, on half of the
+    columns or on all but five (threads, and CTAs of a row that several take,
+    hold nothing else), and one logit far above: their exponentials are 0, so
+    the results are those of -inf there, bit for bit. (f16 has no such values:
+    there the temperature is low.)"""
+    if dtype == "f16":
+        tau *= 1e-5
+    lengths = [4] * 8
+    col, val, z = inputs(8, n, lengths, 21)
+    val, z, c = val.to(DT[dtype]), z.to(DT[dtype]), col.view(8, 4)
+    same = z.clone()
+    for r, size in enumerate(sizes):
+        if kind == "high":
+            same[r, :] = -math.inf
+            z[r, 3] = same[r, 3] = size
+            c[r] = torch.tensor([3, 5, 1, n - 1])
+        else:
+            first = n // 2 if kind == "half" else n - 5
+            z[r, :first], same[r, :first] = -size, -math.inf
+            c[r] = torch.arange(n - 4, n)
+    w = torch.full((8,), tau)
+    loss, dz, err = run(pf, lengths, col, val, z, dtype, w, tau)
+    want_loss, want, _ = run(pf, lengths, col, val, same, dtype, w, tau)
+    assert err == 0 and torch.equal(dz, want) and bool(dz.isfinite().all())
+    assert bool(loss.isfinite().all())
+    if kind != "high":
+        assert torch.equal(loss, want_loss)
+    alone, _, _ = run(pf, lengths, col, val, z, dtype, w, tau, want=("loss",))
+    assert torch.equal(alone, loss)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [700, 40001, 300001])
+def test_rows_of_one_large_value(pf, dtype, n):
+    """Every logit of a row the same finite mask, up to the size at which the
+    formulas in 64 bits still tell log n from 0."""
+    col, val, z = inputs(8, n, [4] * 8, 22)
+    for r, size in enumerate((1e6, 1e7, 3e7, 1e8, 1e9, 3e9, 6e9, 1e10)):
+        z[r, :] = -size
+    check(pf, [4] * 8, col, val, z, dtype)
+    check(pf, [4] * 8, col, val, z, dtype, want=("loss",))
+
+
 def test_plus_infinity_is_nan(pf):
     col, val, z = inputs(2, 300, [3, 3], 4)
     z[0, 7] = math.inf
