@@ -82,6 +82,11 @@ struct Gather {
   }
 };
 
+// Places within a row, counted from its first entry: unsigned, so that steps
+// past the end of a row that ends at the largest signed index do not wrap.
+template <typename IT>
+using Place = typename std::make_unsigned<IT>::type;
+
 // The bounds of the CSR's rows, checked: empty and flagged where the pointers are
 // not non-decreasing within [row_ptr[0], row_ptr[0] + nnz].
 template <typename VT, typename IT>
@@ -146,15 +151,16 @@ spmm_wide_kernel(const WideParams<VT, IT> P, int tpr_log2) {
     bool fetched = true;  // whether col and val are the row's first
     for (int v = blockIdx.y * tpr * Q + sub; v < count; v += gridDim.y * tpr * Q) {
       float acc[Q][8] = {};
-      for (IT i = s; i < e; i += B) {
-        if (!fetched) entries(i, e);
+      const Place<IT> left = (Place<IT>)e - (Place<IT>)s;
+      for (Place<IT> i = 0; i < left; i += B) {
+        if (!fetched) entries(s + (IT)i, e);
         fetched = false;
         Gather<VT, ALIGNED> x[B][Q];
         int delta[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
           if (col[b] >= n) {
-            if (e - i > b) atomicOr(P.err, PF_DEVERR_BOUNDS);
+            if (left - i > b) atomicOr(P.err, PF_DEVERR_BOUNDS);
             col[b] = 0xffffffffu;
             continue;
           }
@@ -226,14 +232,16 @@ sddmm_kernel(const WideParams<VT, IT> P, int wpr_log2) {
   next.check(flag && r0 < P.m, P.err);
   IT s = next.s, e = next.e;
   const uint32_t n = (uint32_t)min(P.n, (int64_t)0xffffffff);
-  uint32_t first = s + mine < e ? (uint32_t)P.col[s + mine] : 0;
+  uint32_t first = e - s > mine ? (uint32_t)P.col[s + mine] : 0;
   next.fetch(r0 + step);
   for (int64_t r = r0; r < P.m; r += step) {
     const DenseRow<VT> Y(P.Y + r * P.ldy, k);
     const int shift = ALIGNED ? 0 : Y.shift, count = Y.count;
     const int first_whole = shift > 0, last_whole = count - 1 - ((k + shift) % 8 != 0);
-    for (IT i = s + mine; i < e; i += wpr) {
-      const uint32_t col = i == s + mine ? first : (uint32_t)P.col[i];
+    const Place<IT> left = (Place<IT>)e - (Place<IT>)s;
+    for (Place<IT> at = mine; at < left; at += wpr) {
+      const IT i = s + (IT)at;
+      const uint32_t col = at == (Place<IT>)mine ? first : (uint32_t)P.col[i];
       if (col >= n) {
         if (lane == 0) atomicOr(P.err, PF_DEVERR_BOUNDS);
         continue;
@@ -278,7 +286,7 @@ sddmm_kernel(const WideParams<VT, IT> P, int wpr_log2) {
     }
     next.check(flag && r + step < P.m, P.err);
     s = next.s, e = next.e;
-    first = s + mine < e ? (uint32_t)P.col[s + mine] : 0;
+    first = e - s > mine ? (uint32_t)P.col[s + mine] : 0;
     next.fetch(r + 2 * step);
   }
 }

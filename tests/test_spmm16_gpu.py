@@ -77,6 +77,34 @@ def test_slice_of_a_larger_matrix(pf):
     check_spmm(pf, [2, 0, 3], 9, 72, "f16", start=5, seed=5)
 
 
+@pytest.mark.parametrize("lengths", [[3, 0, 1, 8, 2, 5, 0, 17, 0], [1, 0, 1, 1, 0], [0, 40], [7],
+                                     [5, 0, 0, 0, 0, 0, 0, 0, 0, 0]])
+@pytest.mark.parametrize("k", [64, 51])
+def test_pointers_that_end_at_the_largest_index(pf, lengths, k):
+    """A slice whose 32-bit pointers end at 2^31 - 1 (col and val are addressed
+    absolutely: only the slice's part of them is there) gives what the same rows
+    give at 0, for the product and for the values' gradient."""
+    dt, m, n, nnz = torch.bfloat16, len(lengths), 12, sum(lengths)
+    start = 2 ** 31 - 1 - nnz
+    col, val = matrix(lengths, n, 14)
+    g = torch.Generator().manual_seed(15)
+    X, dY = torch.randn(n, k, generator=g).to(dt).cuda(), torch.randn(m, k, generator=g).to(dt).cuda()
+    col, val = col.cuda(), val.to(dt).cuda()
+    h = pf.Handle()
+    Y, Z = torch.zeros_like(dY), torch.ones_like(dY)
+    d, e = torch.zeros_like(val), torch.ones_like(val)
+    ptr, at0 = pointers(lengths, start), pointers(lengths)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    pf.spmm(h, m, n, nnz, at0, col, val, X, Y)
+    pf.sddmm(h, m, n, nnz, at0, col, dY, X, d)
+    assert pf.lib.pf_spmm_bf16_i32(h.ptr, m, n, nnz, p(ptr), p(col) - 4 * start, p(val) - 2 * start,
+                                   k, 1.0, p(X), k, 0.0, p(Z), k, None) == 0
+    assert pf.lib.pf_sddmm_bf16_i32(h.ptr, m, n, nnz, p(ptr), p(col) - 4 * start, k, 1.0, p(dY), k,
+                                    p(X), k, 0.0, p(e) - 2 * start, None) == 0
+    assert h.device_error() == 0 and torch.equal(Y, Z) and torch.equal(d, e)
+    h.close()
+
+
 def test_column_agrees_with_spmv(pf):
     lengths = [3, 0, 4, 1]
     col, val = matrix(lengths, 10, 6)
