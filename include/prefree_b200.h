@@ -274,9 +274,11 @@ pf_status pf_distill_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
  * overlap X or W. Deterministic. Asynchronous on `stream`. rows, n, k and
  * groups are at most 2^31 - 1025; stride_w may be 0 (one matrix for all groups).
  * Arrays whose rows start on 16-byte boundaries run on the tensor cores, others
- * on the CUDA cores. A call with few tiles cuts its sums into parts, whose
- * scratch the handle keeps: the first call of its size allocates (make it
- * before a stream capture).                                                 */
+ * on the CUDA cores. A call with few tiles cuts its sums into parts. The scratch
+ * for that (64 KB for each SM) is allocated by the handle's first such call and
+ * kept until the handle is destroyed (captured graphs use it: destroy them
+ * first). A first such call inside a stream capture is refused with
+ * PF_ERR_UNSUPPORTED: make one of any size before.                          */
 pf_status pf_gmm_f16_i32(pf_handle h, int64_t groups, int64_t rows, int64_t n, int64_t k,
                          const int32_t *group_ptr, const uint16_t *X, int64_t ldx,
                          const uint16_t *W, int64_t ldw, int64_t stride_w, int trans_w,

@@ -73,25 +73,33 @@ static int64_t most_tiles(int64_t groups, int64_t rows, int bn) {
   return rows / bn + std::min(groups, rows);
 }
 
-// Scratch for split sums: grows with the largest call, kept by the handle.
+// Scratch for split sums: tiles x parts are at most the SMs (parts_for), so one
+// size serves every call. Made by the handle's first such call and kept as
+// long as the handle: graphs captured since hold its address.
 template <typename IT, typename OT>
 static pf_status split_scratch(pf_handle h, int64_t tiles, GmmTcParams<IT, OT> *p,
                                cudaStream_t st) {
-  const size_t floats = (size_t)tiles * p->parts * 128 * 128, counters = (size_t)tiles * 4;
-  if (floats > h->gmm_partial_cap) {
-    if (h->gmm_partial) cudaFree(h->gmm_partial);
-    h->gmm_partial = nullptr;
-    h->gmm_partial_cap = 0;
-    PF_CUDA_TRY(cudaMalloc(&h->gmm_partial, floats * sizeof(float)));
-    h->gmm_partial_cap = floats;
-  }
-  if (counters > h->gmm_arrived_cap) {
-    if (h->gmm_arrived) cudaFree(h->gmm_arrived);
-    h->gmm_arrived = nullptr;
-    h->gmm_arrived_cap = 0;
-    PF_CUDA_TRY(cudaMalloc(&h->gmm_arrived, counters * sizeof(unsigned)));
-    PF_CUDA_TRY(cudaMemsetAsync(h->gmm_arrived, 0, counters * sizeof(unsigned), st));
-    h->gmm_arrived_cap = counters;
+  if (!h->gmm_partial) {
+    // (a captured clearing would leave the counters as they are until a replay)
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    PF_CUDA_TRY(cudaStreamIsCapturing(st, &capture));
+    if (capture != cudaStreamCaptureStatusNone) {
+      set_error("the handle's first grouped product with split sums allocates: "
+                "make one before the stream capture");
+      return PF_ERR_UNSUPPORTED;
+    }
+    const size_t sums = sizeof(float) * 128 * 128 * h->num_sms;
+    float *partial = nullptr;
+    PF_CUDA_TRY(cudaMalloc(&partial, sums + h->gmm_counters() * sizeof(unsigned)));
+    h->gmm_arrived = reinterpret_cast<unsigned *>(reinterpret_cast<char *>(partial) + sums);
+    const cudaError_t e =
+        cudaMemsetAsync(h->gmm_arrived, 0, h->gmm_counters() * sizeof(unsigned), st);
+    if (e != cudaSuccess) {
+      cudaFree(partial);
+      h->gmm_arrived = nullptr;
+      PF_CUDA_TRY(e);
+    }
+    h->gmm_partial = partial;
   }
   p->most = tiles;
   p->partial = h->gmm_partial;
@@ -135,7 +143,8 @@ static pf_status launch_tc(pf_handle h, const GmmMaps &maps, GmmTcParams<IT, OT>
 }
 
 // Parts of each sum (of `blocks` blocks of 64): as many as there are CTAs to a
-// tile, of `least` blocks at least, eight parts at most. A join costs about what
+// tile (tiles x parts are at most the SMs: split_scratch relies on it), of
+// `least` blocks at least, eight parts at most. A join costs about what
 // 16 blocks do, more where all 128 x 128 sums of the tile exist (a weight
 // gradient); with more items than CTAs the joins come one after another (256
 // tiles in 4 parts: 82 us instead of 42). 17 rows, n 512, k 4096: 23.0 -> 11.9

@@ -43,12 +43,12 @@ struct pf_handle_s {
   unsigned long long *dist_wait = nullptr;  // step-barrier wait, ns summed over CTAs
   int64_t dist_grid = 0;                    // CTAs of the last fused launch
   int64_t dist_cap = 0;
-  // grouped products with split sums: the parts' sums, and a counter for each
-  // tile and warp (all zero between calls)
+  // grouped products with split sums: the parts' sums (128 x 128 for each SM) and,
+  // behind them, four counters for each SM (all zero between calls). One
+  // allocation, never replaced.
   float *gmm_partial = nullptr;
-  size_t gmm_partial_cap = 0;   // floats
   unsigned *gmm_arrived = nullptr;
-  size_t gmm_arrived_cap = 0;
+  size_t gmm_counters() const { return (size_t)num_sms * 4; }
   // host-call buffers, and the copy stream and events of the pipelined
   // host call (created on first use)
   void *hbuf[5] = {nullptr, nullptr, nullptr, nullptr, nullptr};

@@ -814,7 +814,6 @@ pf_status pf_handle_destroy(pf_handle h) {
   }
   if (h->dist_part) cudaFree(h->dist_part);
   if (h->gmm_partial) cudaFree(h->gmm_partial);
-  if (h->gmm_arrived) cudaFree(h->gmm_arrived);
   if (h->sample_dev) cudaFree(h->sample_dev);
   if (h->sample_host) cudaFreeHost(h->sample_host);
   cudaSetDevice(cur);
@@ -849,7 +848,7 @@ pf_status pf_handle_device_error(pf_handle h, uint32_t *bits, int clear) {
     PF_CUDA_TRY(cudaMemset(h->err, 0, sizeof(unsigned)));
     h->scratch_dirty = true;  // a failed launch may leave counters set
     if (h->gmm_arrived)
-      PF_CUDA_TRY(cudaMemset(h->gmm_arrived, 0, h->gmm_arrived_cap * sizeof(unsigned)));
+      PF_CUDA_TRY(cudaMemset(h->gmm_arrived, 0, h->gmm_counters() * sizeof(unsigned)));
   }
   return PF_OK;
 }

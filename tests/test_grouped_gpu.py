@@ -412,3 +412,59 @@ def test_one_matrix_for_all_groups(pf):
         within(Y, Z.double(), 2 * UNIT["bf16"] * Z.double().abs() + 1e-4)
     assert h.device_error() == 0
     h.close()
+
+
+def test_captured_split_sums_outlive_larger_calls(pf):
+    """A graph of split products (17 rows: 4 tiles of 32 blocks; a gradient
+    over 5000 rows) replayed after larger split calls on the same handle, between
+    other calls that use the same scratch."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    h = pf.Handle()
+    X, W, ptr = r(17, 2048), r(1, 512, 2048), pointers([17])
+    A, B, ptr2 = r(5000, 64), r(5000, 72), pointers([5000])
+    Y, dW = torch.empty(17, 512, dtype=X.dtype, device="cuda"), torch.empty(1, 64, 72, device="cuda")
+
+    def step():
+        pf.grouped_mm(h, ptr, X, W, Y)
+        pf.grouped_wgrad(h, ptr2, A, B, dW)
+
+    step()
+    want = Y.clone(), dW.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    more = [(pointers([3, 0, 300, 1]), r(304, 1000), r(4, 264, 1000)),
+            (pointers([60]), r(60, 4096), r(1, 4096, 4096)),
+            (pointers([1] * 30), r(30, 2048), r(30, 128, 2048))]
+    for p, x, w in more:
+        Z, first = (torch.empty(x.shape[0], w.shape[1], dtype=x.dtype, device="cuda")
+                    for _ in range(2))
+        pf.grouped_mm(h, p, x, w, first)
+        Y.fill_(math.nan)
+        dW.fill_(math.nan)
+        graph.replay()
+        pf.grouped_mm(h, p, x, w, Z)
+        assert torch.equal(Y, want[0]) and torch.equal(dW, want[1]) and torch.equal(Z, first)
+    assert h.device_error() == 0
+    del graph
+    h.close()
+
+
+def test_first_split_call_in_a_capture_is_refused(pf):
+    h = pf.Handle()
+    X = torch.ones(17, 2048, dtype=torch.bfloat16, device="cuda")
+    W, Y = torch.ones(1, 512, 2048, dtype=X.dtype, device="cuda"), torch.zeros(17, 512, dtype=X.dtype,
+                                                                              device="cuda")
+    ptr, graph, other = pointers([17]), torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+    with torch.cuda.graph(graph):
+        with pytest.raises(pf.PfError) as e:
+            pf.grouped_mm(h, ptr, X, W, Y)
+        other += 1.0
+    assert e.value.status == 4
+    graph.replay()  # the capture goes on without it
+    assert other.tolist() == [1.0] * 4 and float(Y.abs().sum()) == 0.0
+    pf.grouped_mm(h, ptr, X, W, Y)
+    assert bool((Y == 2048).all()) and h.device_error() == 0
+    del graph
+    h.close()
