@@ -89,6 +89,12 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   int cur = 0;
   PF_CUDA_TRY(cudaGetDevice(&cur));
   PF_CHECK_ARG(cur == h->device, "handle bound to device %d, current device is %d", h->device, cur);
+  if (n == 0) {
+    // no entries, no gradient; and no slots, by whose release the kernel keeps
+    // its warps within DISTILL_RING rows of one another
+    if (loss) PF_CUDA_TRY(cudaMemsetAsync(loss, 0, m * sizeof(float), st));
+    return PF_OK;
+  }
   DistillParams<VT, IT> p;
   p.m = m;
   p.n = n;
@@ -103,7 +109,6 @@ static pf_status launch_distill(pf_handle h, int64_t m, int64_t n, int64_t nnz, 
   p.dZ = dZ;
   p.lddz = lddz;
   p.inv_tau = (float)(1.0 / temperature);
-  if (n == 0) p.Z = nullptr, p.ldz = p.lddz = 0;  // no row has a piece to copy
   p.err = h->err;
   return dZ ? launch_rows<VT, IT, true>(h, p, st) : launch_rows<VT, IT, false>(h, p, st);
 }

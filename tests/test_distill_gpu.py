@@ -175,6 +175,22 @@ def test_no_columns(pf):
     h.close()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_no_columns_many_rows(pf, dtype):
+    """Far more rows than clusters, so that each would take hundreds."""
+    m = 200000
+    z = torch.empty(m, 0, dtype=DT[dtype], device="cuda")
+    loss, w = torch.full((m,), math.nan, device="cuda"), torch.rand(m, device="cuda")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    h = pf.Handle()
+    for weight, dz in ((None, None), (w, None), (w, torch.empty_like(z))):
+        loss.fill_(math.nan)
+        pf.distill(h, m, 0, 0, torch.zeros(m + 1, dtype=torch.int32, device="cuda"), none,
+                   none.to(z.dtype), z, loss, dz, weight)
+        assert bool((loss == 0).all()) and h.device_error() == 0
+    h.close()
+
+
 @pytest.mark.parametrize("keep", [64, 65, 200])
 @pytest.mark.parametrize("n", [700, 20000])
 def test_kept_around_the_listed_number(pf, keep, n):
