@@ -746,9 +746,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
   __syncwarp();
   __syncthreads();
   if (dead && tid == 0) {  // copies may still be on their way into this CTA
-    for (int s = 0; s < STAGES; ++s)
-      if (!ptx::mbar_wait_bounded(&full[s], 0, 50000000ull))
-        ptx::mbar_wait_bounded(&full[s], 1, 50000000ull);
+    for (int s = 0; s < STAGES; ++s) ptx::mbar_drain(&full[s], 50000000ull);
   }
   __syncthreads();
   // no CTA ends while another one may still send to it

@@ -582,11 +582,13 @@ gmm_tc_kernel(const __grid_constant__ GmmMaps M, const GmmTcParams<IT, OT> P) {
   __syncwarp();
   tc::fence_before_sync();
   __syncthreads();
-  if (dead && tid == 0 && rank == 0) {
-    // copies may still be on their way into this CTA pair's shared memory
-    for (int s = 0; s < Cfg::STAGES; ++s)
-      if (!ptx::mbar_wait_bounded(&full[s], 0, 50000000ull))
-        ptx::mbar_wait_bounded(&full[s], 1, 50000000ull);
+  if (dead && tid == 0) {
+    // copies may still be on their way into this CTA pair's shared memory: the
+    // leader's barriers count both CTAs' whole blocks, each CTA's own its partial ones
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      if (rank == 0) ptx::mbar_drain(&full[s], 50000000ull);
+      if (MODE == GMM_DW) ptx::mbar_drain(&tail[s], 50000000ull);
+    }
   }
   if (CG == 2) tc::cluster_sync();
   tc::fence_after_sync();

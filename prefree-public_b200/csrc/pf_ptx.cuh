@@ -135,6 +135,14 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
   }
 }
 
+// For the end after a wait that gave up: waits, at most about `limit_ns`, for
+// what is still on its way to a barrier, whichever phase it counts for. (A wait
+// for one parity returns at once while the other parity's phase runs.)
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint64_t limit_ns) {
+  mbar_wait_bounded(bar, 0, limit_ns);
+  mbar_wait_bounded(bar, 1, limit_ns);
+}
+
 __device__ __forceinline__ uint64_t policy_evict_first() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
