@@ -441,6 +441,31 @@ def test_another_stream_and_capture(pf):
     h.close()
 
 
+@pytest.mark.parametrize("n", [333, 40001])
+def test_a_replay_writes_loss_and_gradient(pf, n):
+    """A captured call writes both outputs anew at every replay, from the inputs
+    of that time, and flags nothing."""
+    lengths = [8, 0, 70, 1]
+    col, val, z = inputs(4, n, lengths, 16)
+    want = [run(pf, lengths, col, val, x, "bf16")[:2] for x in (z, -z)]
+    ptr, dcol, dval = pointers(lengths), col.int().cuda(), val.to(torch.bfloat16).cuda()
+    zz = z.to(torch.bfloat16).cuda()
+    loss, dz = torch.zeros(4, device="cuda"), torch.zeros_like(zz)
+    h, graph = pf.Handle(), torch.cuda.CUDAGraph()
+    pf.distill(h, 4, n, 79, ptr, dcol, dval, zz, loss, dz)
+    with torch.cuda.graph(graph):
+        pf.distill(h, 4, n, 79, ptr, dcol, dval, zz, loss, dz)
+    for x, (l, d) in zip((z, -z), want):
+        zz.copy_(x)
+        loss.fill_(math.nan)
+        dz.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, l) and torch.equal(dz, d) and h.device_error() == 0
+    del graph
+    h.close()
+
+
 def test_refusals(pf):
     h = pf.Handle()
     ptr = pointers([2, 2])
