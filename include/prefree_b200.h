@@ -225,7 +225,11 @@ pf_status pf_sddmm_bf16_i64(pf_handle h, int64_t m, int64_t n, int64_t nnz,
  * teacher mass where the student has nothing but -inf: loss +inf (times the
  * weight), q = 0. NaN and +inf logits give NaN. Repeated columns add up; a
  * column outside [0, n) is flagged in the device error word and ignored.
- * fp32 arithmetic, the loss's closing terms in double; dZ is rounded once.
+ * Finite logits may be of any size: one of -1e10, or the type's lowest value, has
+ * q = 0 beside ordinary ones, as -inf has. fp32 arithmetic, the loss's closing terms in
+ * double; dZ is rounded once. Made for rows that keep up to some hundreds of
+ * logits: a row's are walked by one warp, and past 64, with dZ asked for, by
+ * all. Waits within the kernel give up after 4 s, which is flagged.
  * Deterministic. Asynchronous on `stream`.                                  */
 pf_status pf_distill_f32_i32(pf_handle h, int64_t m, int64_t n, int64_t nnz,
                              const int32_t *row_ptr, const int32_t *col_idx, const float *val,

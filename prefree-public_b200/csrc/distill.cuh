@@ -17,8 +17,8 @@
 // What bounds it: the bytes of Z (and dZ); the exponentials, one an element for
 // the loss and two with the gradient, at 16 a clock and SM, come next (60 % of
 // that rate with bf16 and the gradient). Measured: 4096 x 131072 bf16 with the
-// gradient 430 us (4.8 TB/s of Z and dZ, 74 % of the copy rate), 2048 x 128000
-// fp32 337 us (92 %), 2048 x 65536 fp32 loss alone 82 us (92 %).
+// gradient 426-439 us (4.9 TB/s of Z and dZ, 75 % of the copy rate), 2048 x 128000
+// fp32 358 us (89 %), 2048 x 65536 fp32 loss alone 85 us (95 %).
 #pragma once
 
 #include "pf_ptx.cuh"

@@ -18,14 +18,15 @@
 // Tiles are found on the device from group_ptr (GroupWalk), by each role for
 // itself.
 //
-// Measured: 16384 rows, one group, n 4096, k 2048, bf16: 160-166 us alone
-// (1660-1720 TFLOP/s; cuBLAS's product of the same size 164-171), 207 us in a
-// long run under the power cap (cuBLAS 201-208); 16 groups of 1024 rows 170-178
-// and 230 us; 64 groups of 128 rows, 2048 x 2048: 102-113 us, 82 us of it the
-// weights' bytes. Large products are bound by the tensor cores and the power
-// cap, products of few rows by the weights' bytes, gradients of few rows by
-// their own: 64 of 2048 x 2048 over 64 rows each take 140 us, as does setting
-// those bytes to zero.
+// Measured: 16384 rows, one group, n 4096, k 2048, bf16: 160-183 us in short
+// bursts (cuBLAS's product of the same size 1-2 % less in the same call), 207-213
+// us in a long run under the power cap (cuBLAS 201-211); 16 groups of 1024 rows
+// 170-203 and 230-236 us, 16 uneven ones 252-259; 64 groups of 128 rows, 2048 x
+// 2048: 102-113 us, 82 us of it the weights' bytes. Large products are bound by
+// the tensor cores and the power cap (what uneven groups cost beyond is open),
+// products of few rows by the weights' bytes, gradients of few rows by their own:
+// 64 of 2048 x 2048 over 64 rows each take 140-148 us, setting those bytes to
+// zero 140.
 //
 // DW: rows past a group's end belong to the next group and must not meet the
 // sum (0 * NaN is NaN). A group's last, partial block is announced to a warp of

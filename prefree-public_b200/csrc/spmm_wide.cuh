@@ -7,8 +7,8 @@
 // dense row. Products of 16-bit values are exact in fp32 (alpha is multiplied
 // into the SpMM's values first); sums are in fp32 in the row's order (the same
 // bits on every run) and rounded once. Measured: 8192 rows of eight non-zeros,
-// 2048 columns, 54 us (5.3 TB/s, 81 % of the copy rate); 62259 rows of one
-// non-zero 78 us; the values' gradient of the former 70 us.
+// 2048 columns, 57 us (5.3 TB/s, 80 % of the copy rate); 62259 rows of one
+// non-zero 79 us; the values' gradient of the former 56 us.
 #pragma once
 
 #include "pf_values.cuh"
@@ -35,7 +35,7 @@ struct WideParams {
 // it lies in; Y's pieces give the columns that a thread holds, and X's columns
 // for one of them lie in two of X's pieces, `d` elements further. The second
 // piece is the neighbour thread's first (a hit in L1). (Elements one by one, or
-// pairs in 4-byte words, took 127 and 142 us instead of 41 for the gradients of
+// pairs in 4-byte words, took 127 and 142 us instead of 41-43 for the gradients of
 // 3001 tokens of four slots, 1531 columns.) Elements of neighbours are never
 // stored, and masked where they would be summed.
 template <typename VT>
