@@ -6,9 +6,11 @@
 //   p_j = exp(t_j / tau - Lt),  Lt = log sum_{j in S} exp(t_j / tau)
 //   q_i = exp(z_i / tau - Lz),  Lz = log sum_{all i}  exp(z_i / tau)
 //   loss = w * sum_{j in S} p_j (log p_j - log q_j)
-//        = w * ((sum_j p_j (t_j - z_j) - max t + max z) / tau
+//        = w * (sum_j p_j ((t_j - max t) + (max z - z_j)) / tau
 //               - log sum_j exp((t_j - max t) / tau)
 //               + log sum_i exp((z_i - max z) / tau))
+// (in differences of the row's own values: what all of a row is moved by, a
+// mask's -1e20 for one, leaves no rounding)
 //   dZ_i = (w / tau) * (q_i - sum_{j in S, col_j = i} p_j)
 // An entry with p_j = 0 adds nothing whatever z_j is. A row without teacher
 // mass (no entry, or all of them -inf) and a row of weight 0 have loss 0 and
@@ -17,7 +19,7 @@
 // What bounds it: the bytes of Z (and dZ); the exponentials, one an element for
 // the loss and two with the gradient, at 16 a clock and SM, come next (60 % of
 // that rate with bf16 and the gradient). Measured: 4096 x 131072 bf16 with the
-// gradient 426-439 us (4.9 TB/s of Z and dZ, 75 % of the copy rate), 2048 x 128000
+// gradient 425-439 us (4.9 TB/s of Z and dZ, 75 % of the copy rate), 2048 x 128000
 // fp32 358 us (89 %), 2048 x 65536 fp32 loss alone 85 us (95 %).
 #pragma once
 
@@ -87,6 +89,28 @@ constexpr uint64_t DISTILL_WAIT_NS = 4000000000ull;
 constexpr int DISTILL_MAX_C = 8;    // CTAs of a cluster
 constexpr int DISTILL_LIST = 64;    // entries of a row that the teacher's warp lists
 constexpr int DISTILL_RING = 16;    // rows whose barriers and results are kept apart
+// What the entries of a lane or CTA add to the loss's sum: p times (t - max t) +
+// (ref - z), ref the largest z met so far. A larger ref adds the sum of p times
+// the difference, so that no term but the teacher's, which is small, is negative.
+struct EntrySum {
+  float v, p, ref;
+};
+__device__ __forceinline__ float raised(const EntrySum &s, float ref) {
+  return s.p == 0.0f || ref == s.ref ? s.v : s.v + s.p * (ref - s.ref);
+}
+// p, t - max t and z of one entry
+__device__ __forceinline__ float entry_term(float p, float t, float z, float ref) {
+  return z == -INFINITY ? INFINITY : p * (t + (ref - z));
+}
+// the warp's sums of a (in lane 0) and b (in lane 16)
+__device__ __forceinline__ float warp_sum2(float a, float b) {
+  const bool low = (threadIdx.x & 16) == 0;
+  float v = (low ? a : b) + __shfl_xor_sync(~0u, low ? b : a, 16);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
+}
+
 // 2^(scale (x - m)) is taken as 2^(scale x - ms), ms = scale m rounded, and one
 // more factor corrects that rounding, which a whole sum shares: a power within
 // 1/2 of 0 as long as |ms| is at most 2^24. (From 2^31 on the power leaves fp32's
@@ -188,7 +212,7 @@ __device__ __forceinline__ void subtract_many(const DistillParams<VT, IT> &P, co
 // i + 2 after it has joined row i + 1, to which every reader of row i has sent.
 //
 // A second warp of its own deals with the teacher: the softmax of the row's
-// entries, sum_j p_j (t_j - z_j) over those of the CTA's slice (whose z is in
+// entries, the loss's sum over those of the CTA's slice (whose z is in
 // shared memory), and, one row behind, the loss and the gradient q - p at the
 // entries' columns, written over what the others stored. Nothing in the common
 // case waits for it but the release of the slots, which also keeps it within
@@ -206,7 +230,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
   __shared__ SoftmaxState parts[2][DISTILL_MAX_C * NW];
   __shared__ SoftmaxState student[DISTILL_RING];  // a row's joined statistics
   __shared__ float2 told_as[DISTILL_RING];        // tm; weight / tau / sum of exponentials
-  __shared__ float2 dots[DISTILL_RING][DISTILL_MAX_C];
+  __shared__ float2 dots[DISTILL_RING][DISTILL_MAX_C][2];  // v and ref; p
   __shared__ uint32_t seen[GRAD ? 512 : 1];  // the teacher's warp's: columns met
   __shared__ uint64_t full[STAGES], empty[STAGES], joined[2];
   __shared__ uint64_t told[DISTILL_RING], heard[DISTILL_RING], dotted[DISTILL_RING];
@@ -339,7 +363,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
     // closing arithmetic is in double
     struct {
       int64_t r = -1;
-      float w, d, as, am, qs, qm;
+      float w, d, as, qs;
     } term;
     int terms = 0;
     auto flush_terms = [&] {
@@ -348,7 +372,7 @@ distill_kernel(const DistillParams<VT, IT> P) {
         if (term.as != 0.0f && term.qs == 0.0f) v = (double)term.w * INFINITY;
         else if (term.as != 0.0f)
           v = (double)term.w *
-              (((double)term.d - (double)term.am + (double)term.qm) * (double)P.inv_tau +
+              ((double)term.d * (double)P.inv_tau +
                log((double)term.qs / (double)term.as));
         P.loss[term.r] = (float)v;
       }
@@ -400,15 +424,16 @@ distill_kernel(const DistillParams<VT, IT> P) {
       if (lossy) {
         if (!wait(&dotted[ring], phase)) return false;
         float d = 0.0f;
-        for (int k = 0; k < (int)C; ++k) d += dots[ring][k].x;
+        for (int k = 0; k < (int)C; ++k) {
+          const float2 v = dots[ring][k][0];
+          d += raised(EntrySum{v.x, dots[ring][k][1].x, v.y}, q.m);
+        }
         if (lane == terms) {
           term.r = last.r;
           term.w = last.w;
           term.d = d;
           term.as = last.a.s;
-          term.am = last.a.m;
           term.qs = q.s;
-          term.qm = q.m;
         }
         if (++terms == 32) flush_terms();
       }
@@ -469,10 +494,11 @@ distill_kernel(const DistillParams<VT, IT> P) {
         __syncwarp();
       }
 
-      // sum of p (t - z) over the entries of this CTA's slices. p = 0 adds nothing,
-      // infinite or not.
+      // the sum over the entries of this CTA's slices. p = 0 adds nothing, infinite
+      // or not.
       const float one = 1.0f / a.s;
-      float d = 0.0f, z_[U];
+      EntrySum sum{0.0f, 0.0f, -INFINITY};
+      float z_[U];
       bool own[U] = {};
       for (int c = 0; c < chunks; ++c, ++it) {
         const uint32_t s = it % STAGES;
@@ -490,15 +516,17 @@ distill_kernel(const DistillParams<VT, IT> P) {
             own[u] = true;
           }
         }
-        if (end - first > DISTILL_LIST)
+        if (P.loss && end - first > DISTILL_LIST)
           for (int64_t i = first + DISTILL_LIST + lane; i < end; i += 32) {
             uint32_t cc;
             float t;
             entry(i, &cc, &t);
             const uint32_t at = cc + (uint32_t)shift, vv = at / VE - v0;
-            const float p = power(t);
-            if (t != -INFINITY && vv < (uint32_t)PIECE && p != 0.0f)
-              d += p * one * (t - to_f32(slot[vv * VE + at % VE]));
+            const float p = power(t) * one;
+            if (t != -INFINITY && vv < (uint32_t)PIECE && p != 0.0f) {
+              const float z = to_f32(slot[vv * VE + at % VE]), ref = fmaxf(sum.ref, z);
+              sum = EntrySum{raised(sum, ref) + entry_term(p, t - a.m, z, ref), sum.p + p, ref};
+            }
           }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&empty[s]);
@@ -511,12 +539,23 @@ distill_kernel(const DistillParams<VT, IT> P) {
         }
       if (!ok) break;
       if (P.loss) {
+        float ref = sum.ref;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (own[u] && p_[u] != 0.0f) d += p_[u] * one * (t_[u] - z_[u]);
-        d = warp_sum(d);
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&dotted[ring], C * 8);
-        if (lane == 0) send8(&dots[ring][rank], &dotted[ring], 0, __float_as_uint(d), 0);
+          if (own[u] && p_[u] * one != 0.0f) ref = fmaxf(ref, z_[u]);
+        ref = warp_max(ref);
+        float v = raised(sum, ref);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (own[u] && p_[u] * one != 0.0f) {
+            v += entry_term(p_[u] * one, t_[u] - a.m, z_[u], ref);
+            sum.p += p_[u] * one;
+          }
+        v = warp_sum2(v, sum.p);
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&dotted[ring], C * 16);
+        if (lane % 16 == 0)
+          send8(&dots[ring][rank][lane / 16], &dotted[ring], 0, __float_as_uint(v),
+                __float_as_uint(ref));
         __syncwarp();
       }
       if (rows_in > 0) ok = finish();

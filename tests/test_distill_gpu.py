@@ -320,6 +320,44 @@ def test_rows_of_one_large_value(pf, dtype, n):
     check(pf, [4] * 8, col, val, z, dtype, want=("loss",))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tau", [0.7, 2.0])
+@pytest.mark.parametrize("side", ["student", "teacher", "both"])
+@pytest.mark.parametrize("n,keep", [(64, 4), (700, 64), (700, 200), (40001, 64), (300001, 300)])
+def test_only_differences_count(pf, dtype, tau, side, n, keep):
+    """Rows far from 0: rows of one large finite value (nothing left by a mask),
+    and rows of multiples of a step, large enough that they are exact, moved by
+    a multiple of it. Loss and gradient are those of the rows moved back, where
+    the formulas are evaluated. The loss's error: EPS of the two logarithms and
+    of the sums of p (max z - z) and p (max t - t) over tau, which do not change
+    with the move."""
+    steps = [0.0] * 4 + [2.0 ** -4, 2.0 ** -2, 2.0 ** 7, 2.0 ** 7]
+    moves = [1e6, 1e10, 1e20, 3e38, 2.0 ** 3, 2.0 ** 5, 2.0 ** 14, -2.0 ** 14]
+    g = torch.Generator().manual_seed(n + keep)
+    lengths = [keep] * 8
+    col = torch.cat([torch.randperm(n, generator=g)[:keep] for _ in lengths])
+    z = torch.randint(-12, 13, (8, n), generator=g) * torch.tensor(steps)[:, None]
+    t = torch.randint(-12, 13, (8, keep), generator=g) * torch.tensor(steps)[:, None]
+    move = torch.tensor(moves)[:, None]
+    move[:4] = -move[:4]
+    zm, tm = (z - move, t) if side == "student" else (z, t - move) if side == "teacher" else \
+        (z - move, t - move)
+    zm, tm = zm.to(DT[dtype]), tm.to(DT[dtype])
+    for moved, still, by in ((zm, z, side != "teacher"), (tm, t, side != "student")):
+        back = moved[4:].double() + (move[4:].double() if by else 0.0)
+        assert torch.equal(back, still[4:].double())  # nothing was rounded
+    loss, dz, err = run(pf, lengths, col, tm.flatten(), zm, dtype, None, tau)
+    rl, rd, _, pd = formulas(lengths, col, t.flatten(), z, None, tau)
+    p = torch.softmax(t.double() / tau, 1)
+    far = (p * (z.double().amax(1, keepdim=True) - z.double().gather(1, col.view(8, keep)))).sum(1) + \
+        (p * (t.double().amax(1, keepdim=True) - t.double())).sum(1)
+    assert err == 0
+    within(loss, rl, EPS * (2 + far / tau) + 2.0 ** -23 * rl.abs())
+    within(dz, rd, UNIT[dtype] * rd.abs() + EPS * pd + TINY[dtype])
+    alone, _, _ = run(pf, lengths, col, tm.flatten(), zm, dtype, None, tau, want=("loss",))
+    assert torch.equal(alone, loss)
+
+
 def test_plus_infinity_is_nan(pf):
     col, val, z = inputs(2, 300, [3, 3], 4)
     z[0, 7] = math.inf
